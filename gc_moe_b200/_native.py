@@ -47,6 +47,30 @@ class StageArgs(ctypes.Structure):
             'shared_sf_rows', 'block_m', 'num_tokens', 'hidden', 'num_experts', 'topk')]
 
 
+class NormArgs(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_uint64) for name in (
+        'x', 'residual', 'weight', 'x_q', 'x_sf', 'normed', 'residual_out', 'shared_sf',
+        'x_stride', 'residual_stride', 'normed_stride', 'residual_out_stride')] + [
+        (name, ctypes.c_uint32) for name in ('shared_sf_rows', 'block_m', 'num_tokens', 'hidden')] + [
+        ('residual_f32', ctypes.c_int32), ('weight_f32', ctypes.c_int32), ('eps', ctypes.c_float),
+        ('device', ctypes.c_int32)]
+
+
+class LogitsArgs(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_uint64) for name in ('x', 'weight', 'out', 'x_stride')] + [
+        (name, ctypes.c_uint32) for name in ('num_tokens', 'hidden', 'num_experts', 'planes')] + [
+        ('device', ctypes.c_int32), ('reserved', ctypes.c_uint32)]
+
+
+class RouteArgs(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_uint64) for name in (
+        'logits', 'bias', 'topk_idx', 'topk_weights', 'logits_stride')] + [
+        (name, ctypes.c_uint32) for name in (
+            'num_tokens', 'num_experts', 'topk', 'num_groups', 'topk_groups', 'logit_type', 'sigmoid',
+            'group_by_max', 'renormalize')] + [
+        ('scale', ctypes.c_float), ('device', ctypes.c_int32), ('reserved', ctypes.c_uint32)]
+
+
 class TransformArgs(ctypes.Structure):
     _fields_ = [(name, ctypes.c_uint64) for name in (
         'payload_in', 'payload_out', 'sf_in', 'sf_out', 'block_codes',
@@ -74,6 +98,9 @@ _SIGNATURES = {
     'gcmoe_status_read': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p,
                                          ctypes.POINTER(ctypes.c_uint32)]),
     'gcmoe_stage_inputs': (ctypes.c_int, [ctypes.POINTER(StageArgs), ctypes.c_void_p]),
+    'gcmoe_rms_norm': (ctypes.c_int, [ctypes.POINTER(NormArgs), ctypes.c_void_p]),
+    'gcmoe_router_logits': (ctypes.c_int, [ctypes.POINTER(LogitsArgs), ctypes.c_void_p]),
+    'gcmoe_route': (ctypes.c_int, [ctypes.POINTER(RouteArgs), ctypes.c_void_p]),
     'gcmoe_transform_weights': (ctypes.c_int, [ctypes.POINTER(TransformArgs), ctypes.c_void_p]),
     'gcmoe_launch_static_scratch': (ctypes.c_int, [ctypes.POINTER(Problem), ctypes.POINTER(Buffers), ctypes.c_void_p]),
     'gcmoe_static_scratch_status': (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint32)]),

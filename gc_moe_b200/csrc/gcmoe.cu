@@ -5,9 +5,13 @@
 #include <cstring>
 #include <mutex>
 #include <new>
+#include <type_traits>
 
 #include "../../include/gcmoe.h"
 #include "combine.cuh"
+#include "rms_norm.cuh"
+#include "route.cuh"
+#include "router_logits.cuh"
 #include "stage_inputs.cuh"
 #include "transform_weights.cuh"
 #include "dispatch.cuh"
@@ -732,6 +736,162 @@ extern "C" int gcmoe_stage_inputs(const gcmoe_stage_args* args, void* cuda_strea
     const size_t smem = a.router_logits != 0 ? size_t(a.num_experts) * 4 : 0;
     stage_inputs_kernel<<<a.num_tokens, kStageThreads, smem, static_cast<cudaStream_t>(cuda_stream)>>>(p);
     GCMOE_CUDA(cudaGetLastError());
+    return GCMOE_OK;
+}
+
+// The producers launch on the caller's current device: an address of another one is refused
+// before it reaches a kernel.
+static int check_device(int32_t device) {
+    int current = 0;
+    GCMOE_CUDA(cudaGetDevice(&current));
+    if (device != current)
+        return fail(GCMOE_ERR_INVALID, "the tensors are on device %d, the current device is %d", device, current);
+    return GCMOE_OK;
+}
+
+template <int kChunks, int kResidual>
+static cudaError_t launch_norm(const gcmoe_norm_args& a, const NormParams& p, uint32_t threads, cudaStream_t s) {
+    return launch_dependent(a.weight_f32 ? rms_norm_kernel<kChunks, kResidual, true> : rms_norm_kernel<kChunks, kResidual, false>,
+                            a.num_tokens, threads, 0, s, p, true);
+}
+
+extern "C" int gcmoe_rms_norm(const gcmoe_norm_args* args, void* cuda_stream) {
+    if (args == nullptr) return fail(GCMOE_ERR_INVALID, "null argument");
+    const gcmoe_norm_args& a = *args;
+    if (a.num_tokens == 0) return GCMOE_OK;
+    if (a.num_tokens > 0x7fffffffu) return fail(GCMOE_ERR_INVALID, "too many tokens");
+    if (a.hidden == 0 || a.hidden % 32 || a.hidden > kNormThreads * kNormMaxChunks * 8)
+        return fail(GCMOE_ERR_INVALID, "hidden must be a positive multiple of 32 up to %u", kNormThreads * kNormMaxChunks * 8);
+    if (!(a.eps >= 0.f) || a.eps > 3.0e38f) return fail(GCMOE_ERR_INVALID, "eps must be a finite non-negative number");
+    if (a.x == 0 || a.x % 16 || a.x_stride % 8 || a.weight == 0 || a.weight % 16 || a.x_q == 0 || a.x_q % 8 || a.x_sf == 0 ||
+        a.x_sf % 4)
+        return fail(GCMOE_ERR_INVALID, "norm input or output missing or misaligned");
+    const uint64_t res_vec = a.residual_f32 ? 4 : 8;   // elements in 16 bytes
+    if ((a.residual == 0) != (a.residual_out == 0))
+        return fail(GCMOE_ERR_INVALID, "residual and residual_out go together");
+    if (a.residual % 16 || a.residual_out % 16 || a.residual_stride % res_vec || a.residual_out_stride % res_vec)
+        return fail(GCMOE_ERR_INVALID, "residual rows must be 16-byte aligned");
+    if (a.normed % 16 || a.normed_stride % 8) return fail(GCMOE_ERR_INVALID, "normed rows must be 16-byte aligned");
+    if (a.num_tokens > 1 && ((a.normed != 0 && a.normed_stride < a.hidden) || (a.residual_out != 0 && a.residual_out_stride < a.hidden)))
+        return fail(GCMOE_ERR_INVALID, "output rows overlap");
+    if (a.shared_sf != 0 && (a.hidden % 128 || a.shared_sf % 4 || a.block_m == 0 || a.block_m % 16 ||
+                             uint64_t((a.num_tokens + a.block_m - 1) / a.block_m) * round_up_u32(a.block_m, 128) >
+                                 a.shared_sf_rows))
+        return fail(GCMOE_ERR_INVALID, "shared scale view too small for %u tokens in blocks of %u", a.num_tokens, a.block_m);
+    if (int rc = check_device(a.device)) return rc;
+    NormParams p = {};
+    p.x = reinterpret_cast<const __nv_bfloat16*>(a.x);
+    p.residual = reinterpret_cast<const void*>(a.residual);
+    p.weight = reinterpret_cast<const void*>(a.weight);
+    p.x_q = reinterpret_cast<uint2*>(a.x_q);
+    p.x_sf = reinterpret_cast<uint32_t*>(a.x_sf);
+    p.normed = reinterpret_cast<__nv_bfloat16*>(a.normed);
+    p.residual_out = reinterpret_cast<void*>(a.residual_out);
+    p.shared_sf = reinterpret_cast<uint32_t*>(a.shared_sf);
+    p.x_stride = a.x_stride; p.residual_stride = a.residual_stride;
+    p.normed_stride = a.normed_stride; p.residual_out_stride = a.residual_out_stride;
+    p.shared_sf_rows = a.shared_sf_rows; p.block_m = a.block_m;
+    p.hidden = a.hidden; p.eps = a.eps; p.inv_hidden = 1.0f / float(a.hidden);
+    const uint32_t chunks = a.hidden / 8;
+    uint32_t per_thread = 1;
+    while (per_thread * kNormThreads < chunks) per_thread *= 2;
+    const uint32_t threads = round_up_u32((chunks + per_thread - 1) / per_thread, 32);
+    const int residual = a.residual == 0 ? kNoResidual : a.residual_f32 ? kResidualF32 : kResidualBf16;
+    cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+    auto by_residual = [&](auto chunks_tag) {
+        constexpr int kChunks = decltype(chunks_tag)::value;
+        return residual == kNoResidual ? launch_norm<kChunks, kNoResidual>(a, p, threads, s)
+             : residual == kResidualBf16 ? launch_norm<kChunks, kResidualBf16>(a, p, threads, s)
+                                         : launch_norm<kChunks, kResidualF32>(a, p, threads, s);
+    };
+    GCMOE_CUDA(per_thread == 1 ? by_residual(std::integral_constant<int, 1>())
+               : per_thread == 2 ? by_residual(std::integral_constant<int, 2>())
+               : per_thread == 4 ? by_residual(std::integral_constant<int, 4>())
+                                 : by_residual(std::integral_constant<int, 8>()));
+    return GCMOE_OK;
+}
+
+template <int kPlanes>
+static cudaError_t launch_logits(const LogitsParams& p, cudaStream_t s) {
+    constexpr int kTokens = 4, kExperts = 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((p.num_experts + kExperts - 1) / kExperts, (p.num_tokens + kTokens - 1) / kTokens);
+    cfg.blockDim = dim3(kLogitsThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, logits_fma_kernel<kTokens, kExperts, kPlanes>, p);
+}
+
+extern "C" int gcmoe_router_logits(const gcmoe_logits_args* args, void* cuda_stream) {
+    if (args == nullptr) return fail(GCMOE_ERR_INVALID, "null argument");
+    const gcmoe_logits_args& a = *args;
+    if (a.num_tokens == 0) return GCMOE_OK;
+    if (a.hidden == 0 || a.hidden % 8) return fail(GCMOE_ERR_INVALID, "hidden must be a positive multiple of 8");
+    if (a.num_experts == 0 || a.num_experts > uint32_t(kMaxExperts))
+        return fail(GCMOE_ERR_INVALID, "num_experts must be in 1..%d", kMaxExperts);
+    if (a.planes != 1 && a.planes != 3) return fail(GCMOE_ERR_INVALID, "the router weight has 1 or 3 bf16 planes");
+    if (a.num_tokens > 65535u * 4u) return fail(GCMOE_ERR_INVALID, "at most %u tokens a call", 65535u * 4u);
+    if (a.x == 0 || a.x % 16 || a.x_stride % 8 || a.weight == 0 || a.weight % 16 || a.out == 0 || a.out % 4)
+        return fail(GCMOE_ERR_INVALID, "router input or output missing or misaligned");
+    if (int rc = check_device(a.device)) return rc;
+    LogitsParams p = {};
+    p.x = reinterpret_cast<const __nv_bfloat16*>(a.x);
+    p.weight = reinterpret_cast<const __nv_bfloat16*>(a.weight);
+    p.out = reinterpret_cast<float*>(a.out);
+    p.x_stride = a.x_stride;
+    p.num_tokens = a.num_tokens; p.num_experts = a.num_experts; p.hidden = a.hidden;
+    cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+    GCMOE_CUDA(a.planes == 1 ? launch_logits<1>(p, s) : launch_logits<3>(p, s));
+    return GCMOE_OK;
+}
+
+extern "C" int gcmoe_route(const gcmoe_route_args* args, void* cuda_stream) {
+    if (args == nullptr) return fail(GCMOE_ERR_INVALID, "null argument");
+    const gcmoe_route_args& a = *args;
+    if (a.num_tokens == 0) return GCMOE_OK;
+    if (a.topk == 0 || a.topk > 32) return fail(GCMOE_ERR_INVALID, "topk must be in 1..32");
+    if (a.num_experts == 0 || a.num_experts > uint32_t(kMaxExperts))
+        return fail(GCMOE_ERR_INVALID, "num_experts must be in 1..%d", kMaxExperts);
+    if (a.num_groups == 0 || a.num_groups > 32 || a.num_experts % a.num_groups)
+        return fail(GCMOE_ERR_INVALID, "num_groups must divide num_experts and be at most 32");
+    if (a.topk_groups == 0 || a.topk_groups > a.num_groups)
+        return fail(GCMOE_ERR_INVALID, "topk_groups must be in 1..num_groups");
+    if (a.topk > a.topk_groups * (a.num_experts / a.num_groups))
+        return fail(GCMOE_ERR_INVALID, "topk %u exceeds the %u experts of %u groups", a.topk,
+                    a.topk_groups * (a.num_experts / a.num_groups), a.topk_groups);
+    if (a.logit_type > kLogitF16) return fail(GCMOE_ERR_INVALID, "logits must be f32, bf16 or f16");
+    const uint64_t width = a.logit_type == kLogitF32 ? 4 : 2;
+    if (a.logits == 0 || a.logits % width || a.bias % 4 || a.topk_idx == 0 || a.topk_idx % 8 || a.topk_weights == 0 ||
+        a.topk_weights % 4)
+        return fail(GCMOE_ERR_INVALID, "routing input or output missing or misaligned");
+    if (!(a.scale >= -3.0e38f && a.scale <= 3.0e38f)) return fail(GCMOE_ERR_INVALID, "scale must be finite");
+    RouteParams p = {};
+    p.group_size = a.num_experts / a.num_groups;
+    p.lanes_per_group = 1;
+    while (p.lanes_per_group * 2 * a.num_groups <= 32) p.lanes_per_group *= 2;
+    p.per_lane = (p.group_size + p.lanes_per_group - 1) / p.lanes_per_group;
+    if (p.per_lane > kRouteMaxPerLane)
+        return fail(GCMOE_ERR_UNSUPPORTED, "groups of %u experts in %u groups are too large: at most %u", p.group_size,
+                    a.num_groups, kRouteMaxPerLane * p.lanes_per_group);
+    if (int rc = check_device(a.device)) return rc;
+    p.logits = reinterpret_cast<const void*>(a.logits);
+    p.bias = reinterpret_cast<const float*>(a.bias);
+    p.topk_idx = reinterpret_cast<long long*>(a.topk_idx);
+    p.topk_weights = reinterpret_cast<float*>(a.topk_weights);
+    p.logits_stride = a.logits_stride;
+    p.num_tokens = a.num_tokens; p.num_experts = a.num_experts; p.topk = a.topk;
+    p.num_groups = a.num_groups; p.topk_groups = a.topk_groups;
+    p.logit_type = a.logit_type; p.sigmoid = a.sigmoid; p.group_by_max = a.group_by_max; p.renormalize = a.renormalize;
+    p.scale = a.scale;
+    void (*kernel)(RouteParams) = p.per_lane <= 2 ? route_kernel<2> : p.per_lane <= 4 ? route_kernel<4>
+                                : p.per_lane <= 8 ? route_kernel<8> : p.per_lane <= 16 ? route_kernel<16>
+                                : p.per_lane <= 32 ? route_kernel<32> : route_kernel<64>;
+    const uint32_t grid = (a.num_tokens + kRouteWarps - 1) / kRouteWarps;
+    GCMOE_CUDA(launch_dependent(kernel, grid, kRouteWarps * 32, 0, static_cast<cudaStream_t>(cuda_stream), p, true));
     return GCMOE_OK;
 }
 

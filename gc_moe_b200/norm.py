@@ -1,0 +1,114 @@
+"""``rms_norm_for_gc_moe``: residual addition, RMS norm and the layer's 8-bit
+input format in one kernel.
+
+The reference's operator starts from rows that are already normed and quantised
+(README.md:234-252); this is the step in front of it.  Inference only: the
+results carry no gradient.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple, Optional, Union
+
+import torch
+
+from . import _native
+from .heuristics import get_block_m_for_gc_moe
+
+_FLOATS = (torch.bfloat16, torch.float32)
+
+
+class NormedInputs(NamedTuple):
+    """Results of ``rms_norm_for_gc_moe``."""
+    x: torch.Tensor                      # e4m3 [T, H]
+    x_sf: torch.Tensor                   # int32 [T, ceil(H / 128)], four scale bytes per word
+    normed: Optional[torch.Tensor]       # bf16 [T, H], or None
+    residual: Optional[torch.Tensor]     # x + residual, type of the residual; None without one
+
+
+def _check_rows(t, name: str, shape, dtypes, device: int) -> None:
+    if t.dtype not in dtypes or t.shape != shape or t.get_device() != device or (shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f'{name} must be {" or ".join(str(d)[6:] for d in dtypes)} {list(shape)} on the device of x, '
+                         'contiguous in its last dimension')
+
+
+def _row_stride(t: torch.Tensor, hidden: int) -> int:
+    """Elements between rows; a single row has no stride of its own."""
+    return t.stride(0) if t.shape[0] > 1 else hidden
+
+
+def rms_norm_for_gc_moe(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None,
+                        eps: float = 1e-6, *, normed: Union[bool, torch.Tensor] = True,
+                        residual_out: Optional[torch.Tensor] = None, sym_buffer=None) -> NormedInputs:
+    """``h = x + residual``; ``v = h / sqrt(mean(h * h) + eps) * weight``, all in
+    FP32, from BF16 ``x`` [T, H], ``residual`` [T, H] and ``weight`` [H] (BF16 or
+    FP32 each; H a multiple of 32).
+
+    Returns ``v`` as e4m3 rows with one UE8M0 scale ``2^ceil(log2(amax / 448))``
+    per 32 channels (the layer's input format; rows and words of the workspace
+    when ``sym_buffer`` is given, the rows of ``shared_l1_acts_sf`` included,
+    else new tensors), ``v`` in BF16 when ``normed`` is true (or the tensor to
+    write it to), and ``h`` in the type of ``residual``: in ``residual_out``,
+    which may be ``residual`` itself, or a new tensor.  Rows may have a stride;
+    their starts are 16-byte aligned.  Apart from ``residual_out`` being
+    ``residual``, outputs overlap no input.
+
+    Runs on the current stream and can be captured.
+    """
+    if x.dim() != 2 or x.dtype != torch.bfloat16 or not x.is_cuda or x.stride(1) != 1:
+        raise ValueError('x must be a 2-D CUDA bfloat16 tensor, contiguous in its last dimension')
+    tokens, hidden = shape = x.shape
+    device = x.get_device()
+    if hidden == 0 or hidden % 32:
+        raise ValueError(f'hidden {hidden} must be a positive multiple of 32')
+    if (weight.dtype not in _FLOATS or weight.shape != (hidden,) or weight.get_device() != device
+            or not weight.is_contiguous()):
+        raise ValueError(f'weight must be contiguous bfloat16 or float32 [{hidden}] on the device of x')
+    residual_ptr = residual_stride = residual_out_ptr = residual_out_stride = residual_f32 = 0
+    if residual is not None:
+        _check_rows(residual, 'residual', shape, _FLOATS, device)
+        if residual_out is None:
+            residual_out = torch.empty(shape, dtype=residual.dtype, device=residual.device)
+        elif residual_out is not residual:
+            _check_rows(residual_out, 'residual_out', shape, (residual.dtype,), device)
+        residual_ptr, residual_stride = residual.data_ptr(), _row_stride(residual, hidden)
+        residual_out_ptr, residual_out_stride = residual_out.data_ptr(), _row_stride(residual_out, hidden)
+        residual_f32 = int(residual.dtype is torch.float32)
+    elif residual_out is not None:
+        raise ValueError('residual_out needs a residual')
+    if normed is True:
+        normed = torch.empty(shape, dtype=torch.bfloat16, device=x.device)
+    elif normed is False or normed is None:
+        normed = None
+    else:
+        _check_rows(normed, 'normed', shape, (torch.bfloat16,), device)
+    shared_sf, shared_rows, block_m = None, 0, 0
+    if sym_buffer is None:
+        x_q = torch.empty(shape, dtype=torch.float8_e4m3fn, device=x.device)
+        x_sf = torch.empty((tokens, (hidden + 127) // 128), dtype=torch.int32, device=x.device)
+    else:
+        if sym_buffer.buffer is None:
+            raise ValueError('symmetric buffer has been destroyed')
+        if hidden != sym_buffer.x.shape[1]:
+            raise ValueError(f'x has hidden {hidden}, the workspace {sym_buffer.x.shape[1]}')
+        if tokens > sym_buffer.num_max_tokens_per_rank:
+            raise ValueError(f'{tokens} tokens exceed the workspace capacity {sym_buffer.num_max_tokens_per_rank}')
+        if sym_buffer.x.get_device() != device:
+            raise ValueError('the workspace is on another device than x')
+        x_q, x_sf = sym_buffer.x[:tokens], sym_buffer.x_sf[:tokens]
+        shared_sf = getattr(sym_buffer, 'shared_l1_acts_sf', None)
+        if shared_sf is not None:
+            shared_rows = shared_sf.shape[0]
+            block_m = get_block_m_for_gc_moe(sym_buffer.group.size(), sym_buffer.num_experts,
+                                             sym_buffer.num_max_tokens_per_rank, tokens, sym_buffer.num_topk)
+    args = _native.NormArgs(
+        x.data_ptr(), residual_ptr, weight.data_ptr(), x_q.data_ptr(), x_sf.data_ptr(),
+        0 if normed is None else normed.data_ptr(), residual_out_ptr, 0 if shared_sf is None else shared_sf.data_ptr(),
+        _row_stride(x, hidden), residual_stride, 0 if normed is None else _row_stride(normed, hidden),
+        residual_out_stride, shared_rows, block_m, tokens, hidden, residual_f32,
+        int(weight.dtype is torch.float32), eps, device)
+    code = _native.library().gcmoe_rms_norm(ctypes.byref(args), torch.cuda.current_stream(device).cuda_stream)
+    if code:
+        _native.raise_for(code)
+    return NormedInputs(x_q, x_sf, normed, residual_out)

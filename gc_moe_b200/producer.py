@@ -12,11 +12,14 @@ producer; it has no counterpart function in the reference.
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple, Optional
 
 import torch
 
 from . import _native
 from .heuristics import get_block_m_for_gc_moe
+from .norm import rms_norm_for_gc_moe
+from .router import check_router_weight, check_routing, route_for_gc_moe, router_logits_for_gc_moe
 
 
 def stage_inputs_for_gc_moe(sym_buffer, x: torch.Tensor, router_logits: torch.Tensor | None = None,
@@ -71,3 +74,46 @@ def stage_inputs_for_gc_moe(sym_buffer, x: torch.Tensor, router_logits: torch.Te
     stream = torch.cuda.current_stream().cuda_stream
     _native.raise_for(_native.library().gcmoe_stage_inputs(ctypes.byref(args), ctypes.c_void_p(stream)))
     return block_m
+
+
+class StagedInputs(NamedTuple):
+    """Results of ``stage_normed_inputs_for_gc_moe`` beside the workspace's."""
+    block_m: int                         # of the layer call
+    normed: torch.Tensor                 # bf16 [T, H]: the normed rows
+    residual: Optional[torch.Tensor]     # x + residual, None without a residual
+    logits: torch.Tensor                 # f32 [T, E]
+
+
+def stage_normed_inputs_for_gc_moe(sym_buffer, x: torch.Tensor, norm_weight: torch.Tensor,
+                                   router_weight: torch.Tensor, residual: torch.Tensor | None = None,
+                                   eps: float = 1e-6, *, residual_out: torch.Tensor | None = None,
+                                   scoring: str = 'softmax', bias: torch.Tensor | None = None,
+                                   num_groups: int = 1, topk_groups: int | None = None, group_score: str = 'top2',
+                                   renormalize: bool = True, scale: float = 1.0) -> StagedInputs:
+    """Everything between a decoder layer's attention output ``x`` [T, H] and
+    ``fp8_fp4_gc_moe``: residual addition and RMS norm into the workspace's 8-bit
+    rows (``rms_norm_for_gc_moe``), the router's logits from the BF16 normed rows
+    (``router_logits_for_gc_moe``; ``router_weight`` from
+    ``transform_router_weight_for_gc_moe``), and the workspace's routes
+    (``route_for_gc_moe``, whose options are passed on).  Three kernels on the
+    current stream; can be captured together with the layer call.
+    """
+    # every refusal comes before the first kernel: residual_out may be the residual itself
+    if sym_buffer.buffer is None:
+        raise ValueError('symmetric buffer has been destroyed')
+    if topk_groups is None:
+        topk_groups = num_groups
+    device, experts, topk = x.get_device(), sym_buffer.num_experts, sym_buffer.num_topk
+    check_router_weight(router_weight, sym_buffer.hidden, device)
+    if router_weight.shape[1] != experts:
+        raise ValueError(f'router_weight has {router_weight.shape[1]} experts, the workspace {experts}')
+    check_routing(experts, topk, scoring, bias, num_groups, topk_groups, group_score, scale, device)
+    rows = rms_norm_for_gc_moe(x, norm_weight, residual, eps, residual_out=residual_out, sym_buffer=sym_buffer)
+    tokens = x.shape[0]
+    logits = router_logits_for_gc_moe(rows.normed, router_weight)
+    route_for_gc_moe(logits, topk, scoring=scoring, bias=bias, num_groups=num_groups,
+                     topk_groups=topk_groups, group_score=group_score, renormalize=renormalize, scale=scale,
+                     out=(sym_buffer.topk_idx[:tokens], sym_buffer.topk_weights[:tokens]))
+    block_m = get_block_m_for_gc_moe(sym_buffer.group.size(), experts, sym_buffer.num_max_tokens_per_rank, tokens,
+                                     topk)
+    return StagedInputs(block_m, rows.normed, rows.residual, logits)

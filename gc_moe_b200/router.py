@@ -1,0 +1,158 @@
+"""The router in front of the layer: its product (``router_logits_for_gc_moe``)
+and the choice of experts (``route_for_gc_moe``).
+
+The reference takes ``topk_idx`` and ``topk_weights`` as inputs (README.md:234-252)
+and routes in its tests with a softmax over the k largest logits
+(tests/test_gc_moe.py:130-168).  Inference only: the results carry no gradient.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from . import _native
+
+_LOGIT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_SCORINGS = {'softmax': 0, 'sigmoid': 1}
+_GROUP_SCORES = {'top2': 0, 'max': 1}
+
+
+def transform_router_weight_for_gc_moe(weight: torch.Tensor) -> torch.Tensor:
+    """Router weight [E, H] -> the BF16 planes [P, E, H] that
+    ``router_logits_for_gc_moe`` reads; their sum is the weight.
+
+    A BF16 weight is its own single plane (no copy when it is contiguous).  The
+    24 significant bits of an FP32 weight are three planes of 8: the nearest BF16,
+    the BF16 nearest to what is left, and the rest; planes that would be zero
+    (a BF16 weight stored as FP32) are left out.  Call once per weight, outside
+    graph capture.
+    """
+    if weight.dim() != 2 or weight.dtype not in _LOGIT_TYPES:
+        raise ValueError('router weight must be 2-D bfloat16, float16 or float32')
+    weight = weight.detach()
+    if weight.dtype == torch.bfloat16:
+        return weight.contiguous().unsqueeze(0)
+    if weight.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError('transform weights outside CUDA Graph capture')
+    rest = weight.float()
+    planes = []
+    for _ in range(3):
+        planes.append(rest.to(torch.bfloat16))
+        rest = rest - planes[-1].float()
+    planes = torch.stack(planes)
+    if not bool(torch.isfinite(planes).all()):
+        raise ValueError('router weight has values that are not finite in bfloat16')
+    return planes if bool((planes[1:] != 0).any()) else planes[:1].contiguous()
+
+
+def check_router_weight(router_weight, hidden, device) -> None:
+    if (router_weight.dim() != 3 or router_weight.dtype != torch.bfloat16 or router_weight.shape[0] not in (1, 3)
+            or not 0 < router_weight.shape[1] <= 2048 or router_weight.shape[2] != hidden
+            or router_weight.get_device() != device or not router_weight.is_contiguous() or router_weight.data_ptr() % 16):
+        raise ValueError(f'router_weight must be contiguous, 16-byte aligned bfloat16 [1 or 3, E <= 2048, {hidden}] on '
+                         'the device of x; call transform_router_weight_for_gc_moe first')
+
+
+def router_logits_for_gc_moe(x: torch.Tensor, router_weight: torch.Tensor,
+                             out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """FP32 ``x @ W.T`` [T, E] of BF16 ``x`` [T, H] (rows may have a stride, their
+    starts are 16-byte aligned, H is a multiple of 8) and the planes of
+    ``transform_router_weight_for_gc_moe`` [P, E, H]: exact products, FP32 sums
+    in an order that depends on the sizes alone.
+
+    Runs on the current stream and can be captured.
+    """
+    if x.dim() != 2 or x.dtype != torch.bfloat16 or not x.is_cuda or x.stride(1) != 1:
+        raise ValueError('x must be a 2-D CUDA bfloat16 tensor, contiguous in its last dimension')
+    tokens, hidden = x.shape
+    device = x.get_device()
+    check_router_weight(router_weight, hidden, device)
+    planes, experts = router_weight.shape[:2]
+    if out is None:
+        out = torch.empty((tokens, experts), dtype=torch.float32, device=x.device)
+    elif (out.shape != (tokens, experts) or out.dtype != torch.float32 or out.get_device() != device
+          or not out.is_contiguous()):
+        raise ValueError(f'out must be contiguous float32 [{tokens}, {experts}] on the device of x')
+    args = _native.LogitsArgs(x.data_ptr(), router_weight.data_ptr(), out.data_ptr(),
+                              x.stride(0) if tokens > 1 else hidden, tokens, hidden, experts, planes, device, 0)
+    code = _native.library().gcmoe_router_logits(ctypes.byref(args), torch.cuda.current_stream(device).cuda_stream)
+    if code:
+        _native.raise_for(code)
+    return out
+
+
+def check_routing(experts, topk, scoring, bias, num_groups, topk_groups, group_score, scale, device) -> None:
+    """Raise for options that ``gcmoe_route`` would refuse, before anything is enqueued."""
+    if scoring not in _SCORINGS:
+        raise ValueError(f'scoring must be one of {tuple(_SCORINGS)}, got {scoring!r}')
+    if group_score not in _GROUP_SCORES:
+        raise ValueError(f'group_score must be one of {tuple(_GROUP_SCORES)}, got {group_score!r}')
+    if not (0 < topk <= 32 and 0 < num_groups <= 32 and 0 < topk_groups <= num_groups and 0 < experts <= 2048
+            and experts % num_groups == 0 and topk <= experts // num_groups * topk_groups):
+        raise ValueError(f'invalid routing: top {topk} of {experts} experts in {topk_groups} of {num_groups} groups')
+    lanes = 1 << (32 // num_groups).bit_length() - 1     # of the warp, per group; 64 experts each
+    if experts > 64 * lanes * num_groups:
+        raise NotImplementedError(f'{num_groups} groups of {experts // num_groups} experts are too large: '
+                                  f'at most {64 * lanes} each')
+    if not -3.0e38 <= scale <= 3.0e38:
+        raise ValueError('scale must be finite')
+    if bias is not None and (bias.shape != (experts,) or bias.dtype != torch.float32 or bias.get_device() != device
+                             or not bias.is_contiguous()):
+        raise ValueError(f'bias must be contiguous float32 [{experts}] on the device of the logits')
+
+
+def route_for_gc_moe(logits: torch.Tensor, topk: int, *, scoring: str = 'softmax',
+                     bias: Optional[torch.Tensor] = None, num_groups: int = 1, topk_groups: Optional[int] = None,
+                     group_score: str = 'top2', renormalize: bool = True, scale: float = 1.0,
+                     out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``topk_idx`` int64 [T, k] and ``topk_weights`` FP32 [T, k] of router
+    ``logits`` [T, E] (FP32, BF16 or FP16; rows may have a stride).
+
+    * score: ``sigmoid`` of the logit, or ``softmax`` over all experts of the row;
+    * choice: the k largest ``score + bias`` (``bias`` FP32 [E]), without a bias
+      the k largest logits, descending, ties to the lower expert.  The order is
+      that of the sums in 64 bits;
+    * groups: of ``num_groups`` groups of consecutive experts the ``topk_groups``
+      best are eligible; a group's value is the sum of its two largest
+      ``score + bias`` (``'top2'``; of as many as it has) or the largest of what
+      the choice goes by (``'max'``); ties to the lower group;
+    * weight: the score without the bias, divided by the sum of the row's k if
+      ``renormalize``, times ``scale``.
+
+    An expert whose logit (or bias) is -inf or NaN is never chosen and has no part
+    in the softmax: rows that pad a batch are masked that way.  Where no expert is
+    left the index is -1, which the layer takes as no route, and the weight 0.  A
+    logit of +inf counts as the largest finite float.
+
+    ``out``: the two tensors to write, contiguous, such as the first T rows of
+    the workspace's ``topk_idx`` and ``topk_weights``.  Runs on the current stream
+    and can be captured.
+    """
+    if (logits.dim() != 2 or logits.dtype not in _LOGIT_TYPES or not logits.is_cuda
+            or (logits.shape[1] > 1 and logits.stride(1) != 1)):
+        raise ValueError('logits must be a 2-D CUDA float32, bfloat16 or float16 tensor, contiguous in its last dimension')
+    tokens, experts = logits.shape
+    device = logits.get_device()
+    if topk_groups is None:
+        topk_groups = num_groups
+    check_routing(experts, topk, scoring, bias, num_groups, topk_groups, group_score, scale, device)
+    if out is None:
+        idx = torch.empty((tokens, topk), dtype=torch.int64, device=logits.device)
+        weights = torch.empty((tokens, topk), dtype=torch.float32, device=logits.device)
+    else:
+        idx, weights = out
+        for t, dtype in ((idx, torch.int64), (weights, torch.float32)):
+            if t.shape != (tokens, topk) or t.dtype != dtype or t.get_device() != device or not t.is_contiguous():
+                raise ValueError(f'out must be contiguous int64 and float32 [{tokens}, {topk}] on the device of logits')
+    args = _native.RouteArgs(
+        logits.data_ptr(), 0 if bias is None else bias.data_ptr(), idx.data_ptr(), weights.data_ptr(),
+        logits.stride(0) if tokens > 1 else experts, tokens, experts, topk, num_groups, topk_groups,
+        _LOGIT_TYPES[logits.dtype], _SCORINGS[scoring], _GROUP_SCORES[group_score], int(bool(renormalize)), scale,
+        device, 0)
+    code = _native.library().gcmoe_route(ctypes.byref(args), torch.cuda.current_stream(device).cuda_stream)
+    if code:
+        _native.raise_for(code)
+    return idx, weights

@@ -186,6 +186,78 @@ typedef struct gcmoe_stage_args {
  * Allocates nothing; capturable. */
 int gcmoe_stage_inputs(const gcmoe_stage_args* args, void* cuda_stream);
 
+/* Inputs of gcmoe_rms_norm: device addresses, element counts, and the strides
+ * between rows in elements (the last dimension is contiguous). */
+typedef struct gcmoe_norm_args {
+    uint64_t x;               /* bf16 [T, H], rows 16-byte aligned                    */
+    uint64_t residual;        /* bf16 or f32 [T, H], rows 16-byte aligned, or 0       */
+    uint64_t weight;          /* bf16 or f32 [H], 16-byte aligned                     */
+    uint64_t x_q;             /* out: e4m3 [T, H], contiguous                         */
+    uint64_t x_sf;            /* out: int32 [T, ceil(H/128)], contiguous              */
+    uint64_t normed;          /* out: bf16 [T, H], rows 16-byte aligned, or 0         */
+    uint64_t residual_out;    /* out: type of residual; may be residual itself        */
+    uint64_t shared_sf;       /* out: as in gcmoe_stage_args, or 0                    */
+    uint64_t x_stride, residual_stride, normed_stride, residual_out_stride;
+    uint32_t shared_sf_rows, block_m;
+    uint32_t num_tokens, hidden;
+    int32_t residual_f32, weight_f32;   /* 1: the type is f32, 0: bf16                 */
+    float eps;
+    int32_t device;           /* ordinal of the device the addresses belong to        */
+} gcmoe_norm_args;
+
+/* h = x + residual; v = h / sqrt(mean(h^2) + eps) * weight, in f32, one kernel:
+ * residual_out = h and normed = v rounded to their types, x_q / x_sf = v as e4m3
+ * with one UE8M0 scale per 32 channels (the format of gcmoe_stage_inputs; the
+ * missing bytes of a last word are 127).  H a multiple of 32 up to 32768; with
+ * shared_sf a multiple of 128.  No counterpart in the reference, whose inputs
+ * arrive normed and quantised (README.md:234-252).  Allocates nothing; capturable. */
+int gcmoe_rms_norm(const gcmoe_norm_args* args, void* cuda_stream);
+
+/* Inputs of gcmoe_router_logits. */
+typedef struct gcmoe_logits_args {
+    uint64_t x;               /* bf16 [T, H], rows 16-byte aligned                    */
+    uint64_t weight;          /* bf16 [planes, E, H], contiguous, 16-byte aligned     */
+    uint64_t out;             /* out: f32 [T, E], contiguous                          */
+    uint64_t x_stride;        /* elements between rows of x                           */
+    uint32_t num_tokens, hidden, num_experts, planes;
+    int32_t device;
+    uint32_t reserved;
+} gcmoe_logits_args;
+
+/* out[t][e] = sum over planes p and channels c of x[t][c] * weight[p][e][c], f32
+ * sums.  planes = 1: a bf16 router weight; planes = 3: an f32 weight split into
+ * bf16 terms.  H a multiple of 8, E at most 2048.  The reference takes routing
+ * decisions as inputs (README.md:234-252).  Allocates nothing; capturable. */
+int gcmoe_router_logits(const gcmoe_logits_args* args, void* cuda_stream);
+
+/* Inputs of gcmoe_route. */
+typedef struct gcmoe_route_args {
+    uint64_t logits;          /* f32, bf16 or f16 [T, E], last dimension contiguous   */
+    uint64_t bias;            /* f32 [E], or 0                                        */
+    uint64_t topk_idx;        /* out: int64 [T, k] = GCSymmBuffer.topk_idx            */
+    uint64_t topk_weights;    /* out: f32 [T, k]   = GCSymmBuffer.topk_weights        */
+    uint64_t logits_stride;   /* elements between rows                                */
+    uint32_t num_tokens, num_experts, topk;
+    uint32_t num_groups, topk_groups;
+    uint32_t logit_type;      /* 0: f32, 1: bf16, 2: f16                              */
+    uint32_t sigmoid;         /* 1: scores are sigmoid(l), 0: softmax(l) over the row */
+    uint32_t group_by_max;    /* value of a group: 1 its largest key, 0 the sum of two */
+    uint32_t renormalize;     /* weights are divided by their sum                     */
+    float scale;              /* factor of the weights                                */
+    int32_t device;
+    uint32_t reserved;
+} gcmoe_route_args;
+
+/* The k experts of each token by score + bias (by logit without a bias), among
+ * the topk_groups best of num_groups groups of consecutive experts, descending,
+ * ties to the lower expert; weights from the scores without the bias.  Experts
+ * with a logit or bias of -inf or NaN are never chosen; index -1 and weight 0
+ * where none is left.  E at most 2048, k at most 32, at most 32 groups.  The
+ * reference takes routing decisions as inputs (README.md:234-252; its tests use
+ * a softmax over the k largest logits, tests/test_gc_moe.py:130-168).
+ * Allocates nothing; capturable. */
+int gcmoe_route(const gcmoe_route_args* args, void* cuda_stream);
+
 /* One weight matrix (or one stack of per-expert matrices) of
  * gcmoe_transform_weights: device addresses and element counts. */
 typedef struct gcmoe_transform_args {

@@ -1,0 +1,127 @@
+"""The operators in front of the layer together: norm, router logits and routing
+into a workspace, then the layer call, eagerly and captured in one CUDA graph."""
+import pytest
+import torch
+
+import gc_moe_b200 as G
+from oracle import gcmoe_oracle as O
+
+from _cases import LayerCase
+from test_gpu_norm import _check as check_norm, _inputs as norm_inputs
+from test_gpu_router import _check_logits, _route_reference
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize('tokens', [1, 37, 200])
+@pytest.mark.parametrize('weight', [torch.bfloat16, torch.float32])
+def test_staged_inputs_feed_the_layer(single_rank_group, tokens, weight):
+    e, h, i, k = 16, 1024, 512, 4
+    options = dict(scoring='sigmoid', num_groups=4, topk_groups=2, scale=2.5)
+    case = LayerCase(single_rank_group, e, h, i, k, seed=18)
+    try:
+        x, w, r = norm_inputs(tokens, h, torch.bfloat16, torch.bfloat16, seed=60 + tokens)
+        g = torch.Generator().manual_seed(61)
+        router = (torch.randn((e, h), generator=g) * h ** -0.5).to(weight)
+        bias = torch.randn(e, generator=g) * 0.05
+        planes = G.transform_router_weight_for_gc_moe(router.cuda())
+        xd, wd, rd, bd = x.cuda(), w.cuda(), r.cuda(), bias.cuda()
+        out = torch.empty_like(rd)
+        y = torch.full((tokens, h), float('nan'), dtype=torch.bfloat16, device='cuda')
+
+        def call():
+            staged = G.stage_normed_inputs_for_gc_moe(case.buf, xd, wd, planes, rd, 1e-6, residual_out=out, bias=bd, **options)
+            G.fp8_fp4_gc_moe(y, case.l1, case.l2, case.buf, activation_clamp=10.0)
+            return staged
+
+        staged = call()
+        torch.cuda.synchronize()
+        case.buf.raise_on_device_error()
+        assert staged.block_m == case.block_m(tokens) and staged.residual is out
+        check_norm(G.NormedInputs(case.buf.x[:tokens], case.buf.x_sf[:tokens], staged.normed, out), x, w, r, 1e-6)
+        _check_logits(staged.logits, staged.normed, router)
+        idx, wts = case.buf.topk_idx[:tokens].cpu(), case.buf.topk_weights[:tokens].cpu()
+        want_idx, want_w = _route_reference(staged.logits.cpu(), k, 'sigmoid', bias, 4, 2, 'top2', True, 2.5)
+        assert torch.equal(idx, want_idx) and float((wts.double() - want_w).abs().max()) <= 2.5 * 2.0 ** -16
+        ref = O.moe_layer([case.buf.x[:tokens].cpu()], [case.buf.x_sf[:tokens].cpu()], [idx], [wts], case.q1, case.c1,
+                          case.q2, case.c2, [staged.block_m], clamp=10.0)
+        first = y.cpu().clone()
+        assert torch.isfinite(first.float()).all()
+        assert O.cosine(first, ref.y[0]) >= 0.9999 and O.max_rel_err(first, ref.y[0]) <= 2.0 ** -6
+        graph = torch.cuda.CUDAGraph()
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            with torch.cuda.graph(graph, stream=side):
+                call()
+        other = norm_inputs(tokens, h, torch.bfloat16, torch.bfloat16, seed=70 + tokens)[0].cuda()
+        keep = xd.clone()
+        for _ in range(3):
+            xd.copy_(other)                               # new inputs in the captured tensors ...
+            graph.replay()
+            xd.copy_(keep)                                # ... and the first ones again
+            y.fill_(float('nan'))
+            graph.replay()
+        torch.cuda.synchronize()
+        case.buf.raise_on_device_error()
+        assert torch.equal(y.cpu(), first)
+    finally:
+        case.close()
+
+
+def test_a_batch_padded_with_masked_rows(single_rank_group):
+    """Routing with masked logits stages rows without routes: the layer answers zero for them."""
+    case = LayerCase(single_rank_group, 8, 1024, 512, 2, seed=19)
+    try:
+        x, logits = torch.randn((12, 1024)).to(torch.bfloat16), torch.randn((12, 8))
+        logits[7:] = float('-inf')
+        rows = G.rms_norm_for_gc_moe(x.cuda(), torch.ones(1024, device='cuda'), normed=False, sym_buffer=case.buf)
+        G.route_for_gc_moe(logits.cuda(), 2, out=(case.buf.topk_idx[:12], case.buf.topk_weights[:12]))
+        y = torch.full((12, 1024), float('nan'), dtype=torch.bfloat16, device='cuda')
+        G.fp8_fp4_gc_moe(y, case.l1, case.l2, case.buf, activation_clamp=10.0)
+        torch.cuda.synchronize()
+        case.buf.raise_on_device_error()
+        assert rows.normed is None and bool((y[7:] == 0).all()) and bool((y[:7] != 0).any(-1).all())
+    finally:
+        case.close()
+
+
+def test_results_do_not_depend_on_the_stream():
+    """Two streams at once, each with its own tensors, give what one gives."""
+    x, w, r = (t.cuda() for t in norm_inputs(300, 2048, torch.bfloat16, torch.bfloat16, seed=80))
+    planes = G.transform_router_weight_for_gc_moe(torch.randn((96, 2048), device='cuda') * 0.02)
+
+    def chain(rows):
+        n = G.rms_norm_for_gc_moe(rows, w, r)
+        logits = G.router_logits_for_gc_moe(n.normed, planes)
+        return (n.normed, n.residual, logits, *G.route_for_gc_moe(logits, 6, scoring='sigmoid', num_groups=4, topk_groups=2))
+
+    inputs = [x, x.flip(0).contiguous()]
+    want = [chain(rows) for rows in inputs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in inputs]
+    got = [None, None]
+    for _ in range(10):
+        for s, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[s] = chain(inputs[s])
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+def test_refusals_come_before_the_residual_is_touched(single_rank_group):
+    buf = G.get_symm_buffer_for_gc_moe(single_rank_group, 8, 256, 2, 1024, 512)
+    try:
+        x, w, r = (t.cuda() for t in norm_inputs(4, 1024, torch.bfloat16, torch.bfloat16, seed=90))
+        planes = G.transform_router_weight_for_gc_moe(torch.zeros((8, 1024), dtype=torch.bfloat16, device='cuda'))
+        before = r.clone()
+        for bad in (dict(scoring='tanh'), dict(num_groups=3), dict(bias=torch.zeros(7, device='cuda')), dict(scale=float('nan')),
+                    dict(num_groups=8, topk_groups=1), dict(router_weight=planes[:, :4].contiguous()),
+                    dict(router_weight=planes.float()), dict(x=x.float())):
+            args = {**dict(x=x, router_weight=planes), **bad}
+            with pytest.raises(ValueError):
+                G.stage_normed_inputs_for_gc_moe(buf, args.pop('x'), w, args.pop('router_weight'), r, residual_out=r, **args)
+        torch.cuda.synchronize()
+        assert torch.equal(r, before)
+    finally:
+        buf.destroy()
