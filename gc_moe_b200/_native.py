@@ -100,6 +100,8 @@ _SIGNATURES = {
     'gcmoe_stage_inputs': (ctypes.c_int, [ctypes.POINTER(StageArgs), ctypes.c_void_p]),
     'gcmoe_rms_norm': (ctypes.c_int, [ctypes.POINTER(NormArgs), ctypes.c_void_p]),
     'gcmoe_router_logits': (ctypes.c_int, [ctypes.POINTER(LogitsArgs), ctypes.c_void_p]),
+    'gcmoe_producer_status': (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint32)]),
+    'gcmoe_debug_expire_producer_wait': (ctypes.c_int, [ctypes.c_uint, ctypes.c_void_p]),
     'gcmoe_route': (ctypes.c_int, [ctypes.POINTER(RouteArgs), ctypes.c_void_p]),
     'gcmoe_transform_weights': (ctypes.c_int, [ctypes.POINTER(TransformArgs), ctypes.c_void_p]),
     'gcmoe_launch_static_scratch': (ctypes.c_int, [ctypes.POINTER(Problem), ctypes.POINTER(Buffers), ctypes.c_void_p]),

@@ -148,8 +148,10 @@ class GCSymmBuffer:
 
     def raise_on_device_error(self) -> None:
         """Synchronise and raise RuntimeError if a kernel of any call on this
-        workspace gave up on a bounded wait."""
+        workspace, or of ``router_logits_for_gc_moe`` on its device, gave up on a
+        bounded wait."""
         from . import operator
+        operator.check_producer_status()
         for plan in list(self._plans.values()):
             operator.check_plan_status(plan)
         retired, self._retired_scratch = self._retired_scratch, []

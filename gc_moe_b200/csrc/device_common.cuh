@@ -29,7 +29,7 @@ enum StatusWord : int {
     kStatusWords = 8
 };
 enum StatusCode : uint32_t { kOk = 0, kWaitTimeout = 1, kBadGeometry = 2 };
-enum KernelId : uint32_t { kKernelDispatch = 1, kKernelGemmL1 = 2, kKernelGemmL2 = 3, kKernelCombine = 4 };
+enum KernelId : uint32_t { kKernelDispatch = 1, kKernelGemmL1 = 2, kKernelGemmL2 = 3, kKernelCombine = 4, kKernelLogits = 5 };
 
 struct WaitCtl {
     uint32_t* status;          // global status block

@@ -1,5 +1,6 @@
 // Host side of libgcmoe_sm100.so: argument checks, TMA descriptor encoding,
 // launch configuration and the extern "C" entry points of include/gcmoe.h.
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -812,7 +813,7 @@ extern "C" int gcmoe_rms_norm(const gcmoe_norm_args* args, void* cuda_stream) {
 }
 
 template <int kPlanes>
-static cudaError_t launch_logits(const LogitsParams& p, cudaStream_t s) {
+static cudaError_t launch_logits_fma(const LogitsParams& p, cudaStream_t s) {
     constexpr int kTokens = 4, kExperts = 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((p.num_experts + kExperts - 1) / kExperts, (p.num_tokens + kTokens - 1) / kTokens);
@@ -824,6 +825,69 @@ static cudaError_t launch_logits(const LogitsParams& p, cudaStream_t s) {
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, logits_fma_kernel<kTokens, kExperts, kPlanes>, p);
+}
+
+// Experts per tile and CTAs per tile (the split of K) of the tensor-core form: the pair with
+// the least estimated time, in cycles.  A K block costs the bytes it brings from L2 or the
+// four MMAs, whichever is longer; a launch its waves over the SMs (clusters leave some SMs of
+// a GPC unused), a fixed start and end, and the partial tiles' way through shared memory.
+struct LogitsPlan {
+    uint32_t experts, split;
+};
+static LogitsPlan plan_logits(uint32_t tokens, uint32_t experts, uint32_t blocks) {
+    const uint32_t rows = tokens < kLogitsTileTokens ? tokens : kLogitsTileTokens;
+    const uint64_t token_tiles = (tokens + kLogitsTileTokens - 1) / kLogitsTileTokens;
+    LogitsPlan best = {32, 1};
+    uint64_t least = ~0ull;
+    for (uint32_t n = 32; n <= 256; n *= 2) {
+        if (n > 32 && n / 2 >= experts) break;
+        for (uint32_t split = 1; split <= 8 && split <= blocks; split *= 2) {
+            const uint64_t ctas = token_tiles * ((experts + n - 1) / n) * split;
+            const uint64_t room = split == 8 ? 128 : split == 4 ? 136 : 148;
+            const uint64_t waves = (ctas + room - 1) / room, steps = (blocks + split - 1) / split;
+            const uint64_t bytes = (rows + n) * 128 / 48, mma = 2 * n;
+            const uint64_t time = waves * (steps * (bytes > mma ? bytes : mma) + 2000 + 10 * n + (split > 1 ? rows * n * 4 / 25 : 0));
+            if (time < least) { least = time; best = {n, split}; }
+        }
+    }
+    return best;
+}
+
+template <int kN>
+static int launch_logits_mma(const gcmoe_logits_args& a, uint32_t blocks, uint32_t split, cudaStream_t s) {
+    using Tile = LogitsTile<kN>;
+    LogitsMmaParams p;
+    const uint64_t xdims[2] = {a.hidden, a.num_tokens}, wdims[2] = {a.hidden, uint64_t(a.planes) * a.num_experts};
+    const uint64_t xstride = a.x_stride * 2, wstride = uint64_t(a.hidden) * 2;
+    const uint32_t xbox[2] = {kLogitsBlockK, kLogitsTileTokens}, wbox[2] = {kLogitsBlockK, kN};
+    if (int rc = encode_map(&p.x_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.x, xdims, &xstride, xbox, "router input")) return rc;
+    if (int rc = encode_map(&p.w_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.weight, wdims, &wstride, wbox, "router weight")) return rc;
+    p.out = reinterpret_cast<float*>(a.out);
+    p.num_tokens = a.num_tokens; p.num_experts = a.num_experts;
+    p.k_blocks = (a.hidden + kLogitsBlockK - 1) / kLogitsBlockK; p.planes = a.planes;
+    p.split = split;
+    // the attribute is per device and outlives the call: set once for each
+    static std::atomic<uint64_t> ready{0};
+    const uint64_t bit = 1ull << (a.device & 63);
+    if (!(ready.load() & bit)) {
+        GCMOE_CUDA(cudaFuncSetAttribute(logits_mma_kernel<kN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile::kSmemBytes));
+        ready |= bit;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(split, (a.num_experts + kN - 1) / kN, (a.num_tokens + kLogitsTileTokens - 1) / kLogitsTileTokens);
+    cfg.blockDim = dim3(kLogitsMmaThreads);
+    cfg.dynamicSmemBytes = Tile::kSmemBytes;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = split;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    GCMOE_CUDA(cudaLaunchKernelEx(&cfg, logits_mma_kernel<kN>, p));
+    return GCMOE_OK;
 }
 
 extern "C" int gcmoe_router_logits(const gcmoe_logits_args* args, void* cuda_stream) {
@@ -845,7 +909,51 @@ extern "C" int gcmoe_router_logits(const gcmoe_logits_args* args, void* cuda_str
     p.x_stride = a.x_stride;
     p.num_tokens = a.num_tokens; p.num_experts = a.num_experts; p.hidden = a.hidden;
     cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
-    GCMOE_CUDA(a.planes == 1 ? launch_logits<1>(p, s) : launch_logits<3>(p, s));
+    // Rows that overlap (a broadcast row) have no tensor map.
+    if (a.num_tokens <= kFmaMaxTokens || a.x_stride < a.hidden || a.x_stride >= (1ull << 39)) {
+        GCMOE_CUDA(a.planes == 1 ? launch_logits_fma<1>(p, s) : launch_logits_fma<3>(p, s));
+        return GCMOE_OK;
+    }
+    const uint32_t blocks = (a.hidden + kLogitsBlockK - 1) / kLogitsBlockK * a.planes;
+    const LogitsPlan plan = plan_logits(a.num_tokens, a.num_experts, blocks);
+    switch (plan.experts) {
+        case 32: return launch_logits_mma<32>(a, blocks, plan.split, s);
+        case 64: return launch_logits_mma<64>(a, blocks, plan.split, s);
+        case 128: return launch_logits_mma<128>(a, blocks, plan.split, s);
+        default: return launch_logits_mma<256>(a, blocks, plan.split, s);
+    }
+}
+
+// Status words of the producers' bounded waits after synchronising the stream; a failure is
+// reported once and cleared.
+extern "C" int gcmoe_producer_status(void* cuda_stream, uint32_t* words) {
+    if (words == nullptr) return fail(GCMOE_ERR_INVALID, "null argument");
+    cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+    GCMOE_CUDA(cudaMemcpyFromSymbolAsync(words, g_producer_status, kStatusWords * 4, 0, cudaMemcpyDeviceToHost, s));
+    GCMOE_CUDA(cudaStreamSynchronize(s));
+    if (words[kStatusCode] == 0) return GCMOE_OK;
+    static const uint32_t zero[kStatusWords] = {};
+    GCMOE_CUDA(cudaMemcpyToSymbolAsync(g_producer_status, zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s));
+    return fail(GCMOE_ERR_DEVICE, "device wait gave up: code %u kernel %u site %u block %u observed %u expected %u",
+                words[kStatusCode], words[kStatusKernel], words[kStatusSite], words[kStatusBlock],
+                words[kStatusObserved], words[kStatusExpected]);
+}
+
+__global__ void expire_producer_wait_kernel(uint64_t timeout_ns) {
+    __shared__ uint32_t abort_word;
+    abort_word = 0;
+    WaitCtl ctl;
+    ctl.status = g_producer_status;
+    ctl.failed = nullptr;
+    ctl.abort = &abort_word;
+    ctl.timeout_ns = timeout_ns;
+    ctl.kernel = kKernelLogits;
+    flag_wait_eq(g_producer_status + 7, 0xFFFFFFFFu, ctl, 99);   // word 7 is never written
+}
+
+extern "C" int gcmoe_debug_expire_producer_wait(unsigned timeout_us, void* cuda_stream) {
+    expire_producer_wait_kernel<<<1, 1, 0, static_cast<cudaStream_t>(cuda_stream)>>>(uint64_t(timeout_us) * 1000ull);
+    GCMOE_CUDA(cudaGetLastError());
     return GCMOE_OK;
 }
 

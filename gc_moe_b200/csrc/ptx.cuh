@@ -271,6 +271,41 @@ __device__ __forceinline__ void mma_mxf8f6f4_k128(uint32_t d_tmem, uint64_t a_de
     else GCMOE_MMA_K128("cta_group::1");
 }
 #undef GCMOE_MMA_K128
+// The four K16 MMAs of one K64 stage of BF16 operands (K-major, 128-byte swizzle), f32
+// accumulator: D[tmem] (+)= A[smem] * B[smem].  Both descriptors advance by 32 bytes per
+// step; the first MMA overwrites the accumulator when `accumulate_first` is 0.
+__device__ __forceinline__ void mma_bf16_k64(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                             uint32_t accumulate_first) {
+    asm volatile(
+        "{ .reg .pred p; .reg .b64 da, db;\n"
+        "mov.b64 da, %1; mov.b64 db, %2;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n"
+        "add.u64 da, da, 2; add.u64 db, db, 2;\n"
+        "setp.ne.b32 p, 1, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n"
+        "add.u64 da, da, 2; add.u64 db, db, 2;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n"
+        "add.u64 da, da, 2; add.u64 db, db, 2;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n"
+        "}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate_first)
+        : "memory");
+}
+// Instruction descriptor of kind::f16 with BF16 operands and an f32 accumulator, both
+// operands K-major: D format in 4..5 (1 = f32), A and B formats in 7..9 and 10..12 (1 =
+// bf16), N/8 in 17..22, M/16 in 24..28.
+__device__ __forceinline__ constexpr uint32_t instr_desc_bf16(uint32_t m, uint32_t n) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t cluster_addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(cluster_addr)
+                 : "memory");
+    return v;
+}
 // 32 rows x 16 bytes of shared memory -> 4 TMEM columns, replicated to the
 // four 32-lane quarters (the layout block-scale factors are read from).  For a
 // CTA pair each CTA copies from its own shared memory into its own TMEM.

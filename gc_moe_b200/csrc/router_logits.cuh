@@ -28,6 +28,8 @@ struct LogitsParams {
     uint32_t num_tokens, num_experts, hidden;
 };
 
+constexpr uint32_t kFmaMaxTokens = 8;         // above: the tensor-core form
+
 template <int kTokens, int kExperts, int kPlanes>
 __global__ void __launch_bounds__(kLogitsThreads) logits_fma_kernel(const LogitsParams p) {
     constexpr int kSums = kTokens * kExperts;
@@ -89,6 +91,215 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_fma_kernel(const Logits
 #pragma unroll
         for (uint32_t w = 0; w < kLogitsThreads / 32; ++w) v += partial[w][tid];
         if (t < p.num_tokens && e < p.num_experts) p.out[static_cast<uint64_t>(t) * p.num_experts + e] = v;
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// Tensor-core form, for more than a few tokens: 128 tokens x kN experts per tile, the K
+// blocks (64 channels of one weight plane) of a tile split over the CTAs of a cluster, whose
+// partial tiles are added through distributed shared memory in rank order.
+//
+// The tensor core truncates each addition to its f32 accumulator, always towards zero:
+// measured, the result of a K = 7168 product is 6.7e-6 too small in magnitude (relative
+// error 7.9e-6), growing with the number of MMAs in a chain.  So a chain ends after
+// kChainBlocks K blocks (512 channels: 4.7e-7) and its accumulator is added to f32 sums in
+// registers, rounded to nearest; two accumulators in TMEM keep the MMAs going meanwhile.
+//
+// Warp 0: TMA loads; warp 1: MMAs; warps 2-9: accumulators to registers, then the sums.
+constexpr uint32_t kLogitsMmaThreads = 320;
+constexpr uint32_t kLogitsTileTokens = 128;
+constexpr uint32_t kLogitsBlockK = 64;
+constexpr uint32_t kChainBlocks = 8;
+
+// Where a wait of these launches gave up, for gcmoe_producer_status (they have no plan).
+static __device__ uint32_t g_producer_status[kStatusWords];
+
+template <int kN>
+struct LogitsTile {
+    static constexpr uint32_t kStageBytes = kLogitsTileTokens * 128 + kN * 128;
+    static constexpr uint32_t kStages = kN == 256 ? 4 : kN == 128 ? 6 : 8;
+    static constexpr uint32_t kPitch = kN + 4;                 // floats per row of the partial tile: no bank conflicts
+    static constexpr uint32_t kDataBytes = kStages * kStageBytes;
+    static_assert(kDataBytes >= kLogitsTileTokens * kPitch * 4, "the partial tile reuses the stages");
+    // barriers: full[kStages], empty[kStages], acc_full[2], acc_empty[2], drain; TMEM slot, abort word
+    static constexpr uint32_t kSmemBytes = 1024 + kDataBytes + (2 * kStages + 5) * 8 + 8;
+    static constexpr uint32_t kTmemColumns = 2 * kN < 32 ? 32 : 2 * kN;
+};
+
+struct LogitsMmaParams {
+    CUtensorMap x_map;            // bf16 [T][H], box 64 x 128, 128-byte swizzle
+    CUtensorMap w_map;            // bf16 [P * E][H], box 64 x kN
+    float* out;                   // [T][E]
+    uint32_t num_tokens, num_experts;
+    uint32_t k_blocks, planes;    // ceil(H / 64); planes alternate inside a K block
+    uint32_t split;               // CTAs of a cluster
+};
+
+template <int kN>
+__global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const __grid_constant__ LogitsMmaParams p) {
+    using Tile = LogitsTile<kN>;
+    extern __shared__ uint8_t raw_smem[];
+    const uint32_t base = (ptx::smem_u32(raw_smem) + 1023u) & ~1023u;     // swizzle atoms start on 1 KiB
+    uint8_t* const smem = raw_smem + (base - ptx::smem_u32(raw_smem));
+    const uint32_t bars = base + Tile::kDataBytes;
+    const uint32_t bar_full = bars, bar_empty = bars + 8 * Tile::kStages, bar_acc_full = bars + 16 * Tile::kStages;
+    const uint32_t bar_acc_empty = bar_acc_full + 16, bar_drain = bar_acc_full + 32;
+    volatile uint32_t* const tmem_slot =
+        reinterpret_cast<volatile uint32_t*>(smem + Tile::kDataBytes + (2 * Tile::kStages + 5) * 8);
+    volatile uint32_t* const abort_word = tmem_slot + 1;
+
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = blockIdx.x;                                     // of the cluster: the K range
+    const uint32_t e0 = blockIdx.y * kN, t0 = blockIdx.z * kLogitsTileTokens;
+    const uint32_t blocks = p.k_blocks * p.planes;
+    const uint32_t first = uint32_t(uint64_t(blocks) * rank / p.split);
+    const uint32_t count = uint32_t(uint64_t(blocks) * (rank + 1) / p.split) - first;   // >= 1: split <= blocks
+
+    WaitCtl ctl;
+    ctl.status = g_producer_status;
+    ctl.failed = nullptr;
+    ctl.abort = abort_word;
+    ctl.timeout_ns = 2000000000ull;
+    ctl.kernel = kKernelLogits;
+
+    if (tid == 0) {
+        ptx::prefetch_tensormap(&p.x_map);
+        ptx::prefetch_tensormap(&p.w_map);
+        for (uint32_t i = 0; i < Tile::kStages; ++i) {
+            ptx::mbar_init(bar_full + 8 * i, 1);
+            ptx::mbar_init(bar_empty + 8 * i, 1);
+        }
+        for (uint32_t i = 0; i < 2; ++i) {
+            ptx::mbar_init(bar_acc_full + 8 * i, 1);
+            ptx::mbar_init(bar_acc_empty + 8 * i, 8);
+        }
+        ptx::mbar_init(bar_drain, 1);
+        *abort_word = 0;
+        ptx::fence_mbar_init();
+    }
+    ptx::grid_dependency_wait();
+    // TMEM only after the kernels before this one have ended: none of them can be waiting for it.
+    if (warp == 1) {
+        ptx::tmem_alloc<false>(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), Tile::kTmemColumns);
+        ptx::tmem_relinquish<false>();
+        ptx::tc_fence_before();
+    }
+    __syncthreads();
+    ptx::tc_fence_after();
+    ptx::launch_dependents();
+    const uint32_t tmem = *tmem_slot;
+
+    float acc[kN / 2];                                                    // warps 2-9: one token, half of the experts
+    if (warp == 0) {
+        if (ptx::elect_one()) {
+            uint32_t i = 0;
+            for (; i < count; ++i) {
+                const uint32_t stage = i % Tile::kStages, round = i / Tile::kStages;
+                if (round > 0 && !mbar_wait(bar_empty + 8 * stage, (round - 1) & 1, ctl, 1)) break;
+                const uint32_t block = first + i, kb = block / p.planes, plane = block - kb * p.planes;
+                const uint32_t a = base + stage * Tile::kStageBytes, b = a + kLogitsTileTokens * 128;
+                ptx::mbar_arrive_expect_tx(bar_full + 8 * stage, Tile::kStageBytes);
+                ptx::tma_load_2d(a, &p.x_map, bar_full + 8 * stage, int(kb * kLogitsBlockK), int(t0), ptx::kEvictNormal);
+                ptx::tma_load_2d(b, &p.w_map, bar_full + 8 * stage, int(kb * kLogitsBlockK),
+                                 int(plane * p.num_experts + e0), ptx::kEvictLast);
+            }
+            if (i < count) {
+                // Gave up: the copies in flight land before shared memory is used again.
+                const uint64_t start = ptx::globaltimer_ns();
+                const uint32_t oldest = i > Tile::kStages ? i - Tile::kStages : 0;
+                for (uint32_t j = oldest; j < i; ++j)
+                    while (!ptx::mbar_try_wait(bar_full + 8 * (j % Tile::kStages), (j / Tile::kStages) & 1) &&
+                           ptx::globaltimer_ns() - start < 2000000ull) {}
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (ptx::elect_one()) {
+            constexpr uint32_t idesc = ptx::instr_desc_bf16(kLogitsTileTokens, kN);
+            uint32_t i = 0;
+            for (; i < count; ++i) {
+                const uint32_t stage = i % Tile::kStages, chain = i / kChainBlocks, step = i % kChainBlocks;
+                if (step == 0 && chain >= 2 && !mbar_wait(bar_acc_empty + 8 * (chain & 1), ((chain >> 1) - 1) & 1, ctl, 2)) break;
+                if (!mbar_wait(bar_full + 8 * stage, (i / Tile::kStages) & 1, ctl, 3)) break;
+                ptx::tc_fence_after();
+                const uint32_t a = base + stage * Tile::kStageBytes, b = a + kLogitsTileTokens * 128;
+                ptx::mma_bf16_k64(tmem + (chain & 1) * kN, ptx::smem_desc(a, 1024, true), ptx::smem_desc(b, 1024, true), idesc,
+                                  step != 0);
+                ptx::tc_commit<false>(bar_empty + 8 * stage);
+                if (step == kChainBlocks - 1 || i == count - 1) ptx::tc_commit<false>(bar_acc_full + 8 * (chain & 1));
+            }
+            if (i < count) {
+                // Gave up: the MMAs in flight end before TMEM is freed and shared memory reused.
+                ptx::tc_commit<false>(bar_drain);
+                const uint64_t start = ptx::globaltimer_ns();
+                while (!ptx::mbar_try_wait(bar_drain, 0) && ptx::globaltimer_ns() - start < 2000000ull) {}
+            }
+        }
+        __syncwarp();
+    } else {
+        const uint32_t half = (warp - 2) >> 2;
+        const uint32_t lanes = (warp & 3) << 21;                          // this warp's quarter of the TMEM lanes
+        const uint32_t chains = (count + kChainBlocks - 1) / kChainBlocks;
+#pragma unroll
+        for (int j = 0; j < kN / 2; ++j) acc[j] = 0.f;
+        for (uint32_t chain = 0; chain < chains; ++chain) {
+            // all lanes wait alike; a warp leaves as a whole
+            const bool ready = mbar_wait(bar_acc_full + 8 * (chain & 1), (chain >> 1) & 1, ctl, 4);
+            if (!__all_sync(0xffffffffu, ready)) break;
+            ptx::tc_fence_after();
+            const uint32_t column = tmem + lanes + (chain & 1) * kN + half * (kN / 2);
+#pragma unroll
+            for (int c = 0; c < kN / 2; c += 16) {
+                uint32_t r[16];
+                ptx::tmem_ld16(column + c, r);
+                ptx::tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) acc[c + j] += __uint_as_float(r[j]);
+            }
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(bar_acc_empty + 8 * (chain & 1));
+        }
+    }
+    __syncthreads();
+    // The partial tile replaces the stages: every load has been consumed and every MMA has
+    // ended (the last chain's barrier), or has been drained above.
+    if (warp >= 2) {
+        const bool failed = *abort_word != 0u;
+        const uint32_t half = (warp - 2) >> 2, token = (warp & 3) * 32 + lane;
+        float4* const row = reinterpret_cast<float4*>(smem + (token * Tile::kPitch + half * (kN / 2)) * 4);
+#pragma unroll
+        for (int j = 0; j < kN / 2; j += 4)
+            row[j / 4] = failed ? make_float4(NAN, NAN, NAN, NAN) : make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+    }
+    ptx::cluster_sync();
+    const uint32_t rows = min(kLogitsTileTokens, p.num_tokens - t0);
+    const bool vectors = p.num_experts % 4 == 0;
+    for (uint32_t i = rank * kLogitsMmaThreads + tid; i < rows * (kN / 4); i += p.split * kLogitsMmaThreads) {
+        const uint32_t r = i / (kN / 4), c = i % (kN / 4) * 4;
+        if (e0 + c >= p.num_experts) continue;
+        const uint32_t at = base + (r * Tile::kPitch + c) * 4;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (uint32_t s = 0; s < p.split; ++s) {
+            const float4 v = ptx::ld_cluster_f32x4(ptx::mapa(at, s));
+            sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+        }
+        float* const out = p.out + static_cast<uint64_t>(t0 + r) * p.num_experts + e0 + c;
+        if (vectors) {
+            *reinterpret_cast<float4*>(out) = sum;
+        } else {
+            const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j)
+                if (e0 + c + j < p.num_experts) out[j] = v[j];
+        }
+    }
+    // no CTA leaves while another may still read its partial tile
+    __syncwarp();
+    ptx::cluster_sync();
+    if (warp == 1) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc<false>(tmem, Tile::kTmemColumns);
     }
 }
 

@@ -189,6 +189,13 @@ def check_plan_status(plan: _Plan) -> None:
     _native.raise_for(_native.library().gcmoe_status_read(plan.handle, ctypes.c_void_p(stream), words))
 
 
+def check_producer_status() -> None:
+    """Waits of the launches that have no plan (router logits)."""
+    words = (ctypes.c_uint32 * _native.STATUS_WORDS)()
+    stream = torch.cuda.current_stream().cuda_stream
+    _native.raise_for(_native.library().gcmoe_producer_status(ctypes.c_void_p(stream), words))
+
+
 def check_retired_status(scratch: torch.Tensor) -> None:
     """Status words of a plan that has been evicted (the block starts with them)."""
     words = scratch[:_native.STATUS_WORDS * 4].view(torch.int32).tolist()

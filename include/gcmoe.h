@@ -230,6 +230,16 @@ typedef struct gcmoe_logits_args {
  * decisions as inputs (README.md:234-252).  Allocates nothing; capturable. */
 int gcmoe_router_logits(const gcmoe_logits_args* args, void* cuda_stream);
 
+/* Status words of the bounded waits inside gcmoe_router_logits, after
+ * synchronising `cuda_stream`: GCMOE_ERR_DEVICE if one of the launches on the
+ * current device has given up since the last query (its part of the result is
+ * NaN).  The launches have no plan, so the words live in the library. */
+int gcmoe_producer_status(void* cuda_stream, uint32_t* words);
+
+/* Test hook, as gcmoe_debug_expire_wait: one bounded wait that runs out and is
+ * reported by gcmoe_producer_status. */
+int gcmoe_debug_expire_producer_wait(unsigned timeout_us, void* cuda_stream);
+
 /* Inputs of gcmoe_route. */
 typedef struct gcmoe_route_args {
     uint64_t logits;          /* f32, bf16 or f16 [T, E], last dimension contiguous   */

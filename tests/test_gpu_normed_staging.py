@@ -125,3 +125,24 @@ def test_refusals_come_before_the_residual_is_touched(single_rank_group):
         assert torch.equal(r, before)
     finally:
         buf.destroy()
+
+
+def test_a_wait_that_gives_up_is_reported_once(single_rank_group):
+    """The router's launches have no plan: their status is the library's, and the workspace's check reads it."""
+    import ctypes
+    from gc_moe_b200 import _native
+    lib = _native.library()
+    buf = G.get_symm_buffer_for_gc_moe(single_rank_group, 8, 256, 2, 1024, 512)
+    try:
+        buf.raise_on_device_error()
+        stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+        _native.raise_for(lib.gcmoe_debug_expire_producer_wait(200, stream))
+        with pytest.raises(RuntimeError, match='gave up: code 1 kernel 5'):
+            buf.raise_on_device_error()
+        buf.raise_on_device_error()
+        # and the next product is right
+        x, w = torch.randn((130, 512), device='cuda').to(torch.bfloat16), torch.randn((20, 512), device='cuda').to(torch.bfloat16)
+        _check_logits(G.router_logits_for_gc_moe(x, G.transform_router_weight_for_gc_moe(w)), x, w)
+        buf.raise_on_device_error()
+    finally:
+        buf.destroy()
