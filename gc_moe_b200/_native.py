@@ -9,6 +9,8 @@ from __future__ import annotations
 import ctypes
 import os
 
+import torch
+
 MAX_RANKS = 72
 STATUS_WORDS = 8
 
@@ -128,6 +130,12 @@ def library() -> ctypes.CDLL:
             fn.restype, fn.argtypes = restype, argtypes
         _lib = lib
     return _lib
+
+
+# Handle of the current stream of a device: what torch.cuda.current_stream(device).cuda_stream
+# returns, without building a Stream object (1.3 us less a call, where a launch takes 3).
+current_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def last_error() -> str:

@@ -841,9 +841,9 @@ static LogitsPlan plan_logits(uint32_t tokens, uint32_t experts, uint32_t blocks
     uint64_t least = ~0ull;
     for (uint32_t n = 32; n <= 256; n *= 2) {
         if (n > 32 && n / 2 >= experts) break;
-        for (uint32_t split = 1; split <= 8 && split <= blocks; split *= 2) {
+        for (uint32_t split = 1; split <= 16 && split <= blocks; split *= 2) {
             const uint64_t ctas = token_tiles * ((experts + n - 1) / n) * split;
-            const uint64_t room = split == 8 ? 128 : split == 4 ? 136 : 148;
+            const uint64_t room = split >= 8 ? 128 : split == 4 ? 136 : 148;
             const uint64_t waves = (ctas + room - 1) / room, steps = (blocks + split - 1) / split;
             const uint64_t bytes = (rows + n) * 128 / 48, mma = 2 * n;
             const uint64_t time = waves * (steps * (bytes > mma ? bytes : mma) + 2000 + 10 * n + (split > 1 ? rows * n * 4 / 25 : 0));
@@ -854,27 +854,36 @@ static LogitsPlan plan_logits(uint32_t tokens, uint32_t experts, uint32_t blocks
 }
 
 template <int kN>
-static int launch_logits_mma(const gcmoe_logits_args& a, uint32_t blocks, uint32_t split, cudaStream_t s) {
+static int launch_logits_mma(const gcmoe_logits_args& a, uint32_t split, cudaStream_t s) {
     using Tile = LogitsTile<kN>;
     LogitsMmaParams p;
-    const uint64_t xdims[2] = {a.hidden, a.num_tokens}, wdims[2] = {a.hidden, uint64_t(a.planes) * a.num_experts};
-    const uint64_t xstride = a.x_stride * 2, wstride = uint64_t(a.hidden) * 2;
-    const uint32_t xbox[2] = {kLogitsBlockK, kLogitsTileTokens}, wbox[2] = {kLogitsBlockK, kN};
-    if (int rc = encode_map(&p.x_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.x, xdims, &xstride, xbox, "router input")) return rc;
-    if (int rc = encode_map(&p.w_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.weight, wdims, &wstride, wbox, "router weight")) return rc;
+    p.box_tokens = a.num_tokens < kLogitsTileTokens ? round_up_u32(a.num_tokens, 8) : kLogitsTileTokens;
+    p.wide = a.hidden % kLogitsBlockK == 0;
+    const uint64_t w_rows = uint64_t(a.planes) * a.num_experts, x_pitch = a.x_stride * 2, w_pitch = uint64_t(a.hidden) * 2;
+    const uint64_t k_blocks = a.hidden / kLogitsBlockK;
+    const uint64_t x_dims[3] = {p.wide ? kLogitsBlockK : a.hidden, a.num_tokens, k_blocks};
+    const uint64_t w_dims[3] = {p.wide ? kLogitsBlockK : a.hidden, w_rows, k_blocks};
+    const uint64_t x_strides[2] = {x_pitch, kLogitsBlockK * 2}, w_strides[2] = {w_pitch, kLogitsBlockK * 2};
+    const uint32_t x_box[3] = {kLogitsBlockK, p.box_tokens, Tile::kStageBlocks}, w_box[3] = {kLogitsBlockK, kN, Tile::kStageBlocks};
+    const uint32_t dims = p.wide ? 3 : 2;
+    if (int rc = encode_map(&p.x_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dims, a.x, x_dims, x_strides, x_box, "router input")) return rc;
+    if (int rc = encode_map(&p.w_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dims, a.weight, w_dims, w_strides, w_box, "router weight"))
+        return rc;
     p.out = reinterpret_cast<float*>(a.out);
     p.num_tokens = a.num_tokens; p.num_experts = a.num_experts;
-    p.k_blocks = (a.hidden + kLogitsBlockK - 1) / kLogitsBlockK; p.planes = a.planes;
-    p.split = split;
+    p.k_stages = (a.hidden + kLogitsBlockK * Tile::kStageBlocks - 1) / (kLogitsBlockK * Tile::kStageBlocks);
+    p.planes = a.planes;
+    p.split = split < p.k_stages * p.planes ? split : p.k_stages * p.planes;
     // the attribute is per device and outlives the call: set once for each
     static std::atomic<uint64_t> ready{0};
     const uint64_t bit = 1ull << (a.device & 63);
     if (!(ready.load() & bit)) {
         GCMOE_CUDA(cudaFuncSetAttribute(logits_mma_kernel<kN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile::kSmemBytes));
+        GCMOE_CUDA(cudaFuncSetAttribute(logits_mma_kernel<kN>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         ready |= bit;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(split, (a.num_experts + kN - 1) / kN, (a.num_tokens + kLogitsTileTokens - 1) / kLogitsTileTokens);
+    cfg.gridDim = dim3(p.split, (a.num_experts + kN - 1) / kN, (a.num_tokens + kLogitsTileTokens - 1) / kLogitsTileTokens);
     cfg.blockDim = dim3(kLogitsMmaThreads);
     cfg.dynamicSmemBytes = Tile::kSmemBytes;
     cfg.stream = s;
@@ -882,7 +891,7 @@ static int launch_logits_mma(const gcmoe_logits_args& a, uint32_t blocks, uint32
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = split;
+    attr[1].val.clusterDim.x = p.split;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
@@ -917,10 +926,10 @@ extern "C" int gcmoe_router_logits(const gcmoe_logits_args* args, void* cuda_str
     const uint32_t blocks = (a.hidden + kLogitsBlockK - 1) / kLogitsBlockK * a.planes;
     const LogitsPlan plan = plan_logits(a.num_tokens, a.num_experts, blocks);
     switch (plan.experts) {
-        case 32: return launch_logits_mma<32>(a, blocks, plan.split, s);
-        case 64: return launch_logits_mma<64>(a, blocks, plan.split, s);
-        case 128: return launch_logits_mma<128>(a, blocks, plan.split, s);
-        default: return launch_logits_mma<256>(a, blocks, plan.split, s);
+        case 32: return launch_logits_mma<32>(a, plan.split, s);
+        case 64: return launch_logits_mma<64>(a, plan.split, s);
+        case 128: return launch_logits_mma<128>(a, plan.split, s);
+        default: return launch_logits_mma<256>(a, plan.split, s);
     }
 }
 
@@ -957,6 +966,27 @@ extern "C" int gcmoe_debug_expire_producer_wait(unsigned timeout_us, void* cuda_
     return GCMOE_OK;
 }
 
+template <typename T, int kPerLane>
+static auto route_kernel_of(const RouteParams& p, const gcmoe_route_args& a) -> void (*)(RouteParams) {
+    // Vector loads: every lane of a group has exactly kPerLane experts, and they start on a
+    // multiple of 16 bytes, or of their size if that is less (kPerLane 2 and 4).
+    const uint64_t run = kPerLane * sizeof(T) < 16 ? kPerLane * sizeof(T) : 16;
+    const uint64_t bias_run = kPerLane * 4 < 16 ? kPerLane * 4 : 16;
+    if (kPerLane <= 16 && p.per_lane == kPerLane && (p.per_lane << p.lanes_log2) == p.group_size && a.logits % run == 0 &&
+        a.logits_stride * sizeof(T) % run == 0 && a.bias % bias_run == 0)
+        return route_kernel<T, kPerLane, kPerLane <= 16>;
+    return route_kernel<T, kPerLane, false>;
+}
+template <typename T>
+static auto route_kernel_for(const RouteParams& p, const gcmoe_route_args& a) -> void (*)(RouteParams) {
+    return p.per_lane <= 2    ? route_kernel_of<T, 2>(p, a)
+           : p.per_lane <= 4  ? route_kernel_of<T, 4>(p, a)
+           : p.per_lane <= 8  ? route_kernel_of<T, 8>(p, a)
+           : p.per_lane <= 16 ? route_kernel_of<T, 16>(p, a)
+           : p.per_lane <= 32 ? route_kernel_of<T, 32>(p, a)
+                              : route_kernel_of<T, 64>(p, a);
+}
+
 extern "C" int gcmoe_route(const gcmoe_route_args* args, void* cuda_stream) {
     if (args == nullptr) return fail(GCMOE_ERR_INVALID, "null argument");
     const gcmoe_route_args& a = *args;
@@ -979,12 +1009,12 @@ extern "C" int gcmoe_route(const gcmoe_route_args* args, void* cuda_stream) {
     if (!(a.scale >= -3.0e38f && a.scale <= 3.0e38f)) return fail(GCMOE_ERR_INVALID, "scale must be finite");
     RouteParams p = {};
     p.group_size = a.num_experts / a.num_groups;
-    p.lanes_per_group = 1;
-    while (p.lanes_per_group * 2 * a.num_groups <= 32) p.lanes_per_group *= 2;
-    p.per_lane = (p.group_size + p.lanes_per_group - 1) / p.lanes_per_group;
+    p.lanes_log2 = 0;
+    while ((2u << p.lanes_log2) * a.num_groups <= 32) ++p.lanes_log2;
+    p.per_lane = (p.group_size + (1u << p.lanes_log2) - 1) >> p.lanes_log2;
     if (p.per_lane > kRouteMaxPerLane)
         return fail(GCMOE_ERR_UNSUPPORTED, "groups of %u experts in %u groups are too large: at most %u", p.group_size,
-                    a.num_groups, kRouteMaxPerLane * p.lanes_per_group);
+                    a.num_groups, kRouteMaxPerLane << p.lanes_log2);
     if (int rc = check_device(a.device)) return rc;
     p.logits = reinterpret_cast<const void*>(a.logits);
     p.bias = reinterpret_cast<const float*>(a.bias);
@@ -993,11 +1023,11 @@ extern "C" int gcmoe_route(const gcmoe_route_args* args, void* cuda_stream) {
     p.logits_stride = a.logits_stride;
     p.num_tokens = a.num_tokens; p.num_experts = a.num_experts; p.topk = a.topk;
     p.num_groups = a.num_groups; p.topk_groups = a.topk_groups;
-    p.logit_type = a.logit_type; p.sigmoid = a.sigmoid; p.group_by_max = a.group_by_max; p.renormalize = a.renormalize;
+    p.sigmoid = a.sigmoid; p.group_by_max = a.group_by_max; p.renormalize = a.renormalize;
     p.scale = a.scale;
-    void (*kernel)(RouteParams) = p.per_lane <= 2 ? route_kernel<2> : p.per_lane <= 4 ? route_kernel<4>
-                                : p.per_lane <= 8 ? route_kernel<8> : p.per_lane <= 16 ? route_kernel<16>
-                                : p.per_lane <= 32 ? route_kernel<32> : route_kernel<64>;
+    auto kernel = a.logit_type == kLogitF32    ? route_kernel_for<float>(p, a)
+                  : a.logit_type == kLogitBf16 ? route_kernel_for<__nv_bfloat16>(p, a)
+                                               : route_kernel_for<__half>(p, a);
     const uint32_t grid = (a.num_tokens + kRouteWarps - 1) / kRouteWarps;
     GCMOE_CUDA(launch_dependent(kernel, grid, kRouteWarps * 32, 0, static_cast<cudaStream_t>(cuda_stream), p, true));
     return GCMOE_OK;

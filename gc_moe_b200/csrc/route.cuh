@@ -12,22 +12,28 @@
 // no expert is left gets index -1 (no route) and weight 0.  A logit of +inf counts as the
 // largest finite float.
 //
-// The order is that of the keys computed in 64 bits, whatever the sums' order in 32: keys
-// are kept as f32 with a bound on their error, and a round in which two candidates lie
-// within that bound of each other computes those candidates again in f64.
+// The order is that of the keys computed in 64 bits, whatever the sums' order in 32: a row
+// is chosen by f32 keys with a bound on their error, and chosen again by f64 keys where two
+// neighbours in the order lie within that bound of each other (exact ties among them).
 //
-// One warp per token; each of a group's lanes holds consecutive experts in registers, as
-// integers that order like the floats (0 = not eligible), so that a round of the selection
-// is one redux.max, a ballot, and a rescan of the winner's registers.  Bound by
-// instruction issue for many tokens and by latency for few; the bytes (E logits in, 12 k
-// out) are small beside both.
+// One warp per token; each of a group's lanes holds consecutive experts in registers.  Keys
+// are integers that order like the floats (0 = not eligible) whose lowest bits are replaced
+// by the expert's place in its lane, so that equal keys go to the lower expert and a
+// minimum or maximum moves key and expert together: a lane's list is sorted with two
+// instructions per comparison, and a round of the selection is one redux.max, a ballot and a
+// shift of the winner's list.  The replaced bits count as part of the keys' error.
+//
+// Bound by instruction issue for many tokens and by latency for few; the bytes (E logits
+// in, 12 k out) are small beside both.
 #pragma once
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <cfloat>
+#include <cstring>
 #include <stdint.h>
+#include <type_traits>
 
 #include "device_common.cuh"
 #include "ptx.cuh"
@@ -46,16 +52,16 @@ struct RouteParams {
     uint64_t logits_stride;       // elements between rows
     uint32_t num_tokens, num_experts, topk;
     uint32_t num_groups, topk_groups, group_size;
-    uint32_t lanes_per_group;     // power of two; lanes_per_group * num_groups <= 32
-    uint32_t per_lane;            // experts of a lane: ceil(group_size / lanes_per_group)
-    uint32_t logit_type, sigmoid, group_by_max, renormalize;
+    uint32_t lanes_log2;          // lanes of a group, a power of two; lanes * num_groups <= 32
+    uint32_t per_lane;            // experts of a lane: ceil(group_size / lanes)
+    uint32_t sigmoid, group_by_max, renormalize;
     float scale;
 };
 
 // Integers in the order of the floats; -0 and +0 are the same, and no float maps to 0.
 __device__ __forceinline__ uint32_t order_f32(float v) {
     const uint32_t b = __float_as_uint(v + 0.0f);
-    return b ^ (b & 0x80000000u ? 0xffffffffu : 0x80000000u);
+    return b ^ (uint32_t(int32_t(b) >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float unorder_f32(uint32_t u) {
     return __uint_as_float(u ^ (u & 0x80000000u ? 0x80000000u : 0xffffffffu));
@@ -65,49 +71,169 @@ __device__ __forceinline__ uint64_t order_f64(double v) {
     return b ^ (b >> 63 ? 0xffffffffffffffffull : 0x8000000000000000ull);
 }
 
-// A row's logit, and whether the expert can be chosen at all.
+template <typename T>
+__device__ __forceinline__ float logit_f32(T v) {
+    if constexpr (sizeof(T) == 4) return v;
+    else return static_cast<float>(v);
+}
+__device__ __forceinline__ float min_nan(float a, float b) {          // NaN if either is
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// NaN stays NaN, +inf becomes the largest finite float.
+__device__ __forceinline__ float clean_logit(float l) { return min_nan(l, FLT_MAX); }
+
+// A row's logit, its bias, and whether the expert can be chosen at all (false for NaN too).
+template <typename T>
 __device__ __forceinline__ bool load_logit(const RouteParams& p, uint64_t row, uint32_t e, float& l, float& b) {
-    if (p.logit_type == kLogitF32) l = static_cast<const float*>(p.logits)[row + e];
-    else if (p.logit_type == kLogitBf16) l = __bfloat162float(static_cast<const __nv_bfloat16*>(p.logits)[row + e]);
-    else l = __half2float(static_cast<const __half*>(p.logits)[row + e]);
-    l = fminf(l, isnan(l) ? l : FLT_MAX);
+    l = clean_logit(logit_f32(static_cast<const T*>(p.logits)[row + e]));
     b = p.bias != nullptr ? p.bias[e] : 0.f;
-    return l > -INFINITY && b > -INFINITY;            // false for NaN too
+    return l > -INFINITY && b > -INFINITY;
 }
 
+// kCount consecutive values at an address aligned to 16 bytes, or to all of them.
+template <int kCount, typename T>
+__device__ __forceinline__ void load_run(const T* from, float (&v)[kCount]) {
+    constexpr int kBytes = kCount * int(sizeof(T));
+    using Vec = std::conditional_t<kBytes % 16 == 0, uint4, std::conditional_t<kBytes == 8, uint2, uint32_t>>;
+    static_assert(kBytes % sizeof(Vec) == 0, "a run is whole vectors");
+    constexpr int kPer = int(sizeof(Vec) / sizeof(T));
+#pragma unroll
+    for (int i = 0; i < kCount / kPer; ++i) {
+        const Vec raw = __ldg(reinterpret_cast<const Vec*>(from) + i);
+        T part[kPer];
+        memcpy(part, &raw, sizeof(Vec));
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) v[i * kPer + j] = logit_f32(part[j]);
+    }
+}
+
+// For keys: approximate exponential (2^(-l log2 e)) and reciprocal; the bound on the error
+// below covers them.
+__device__ __forceinline__ float sigmoid_approx(float l) {
+    float z;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(z) : "f"(l * -1.44269504f));
+    return ptx::rcp_approx_ftz(1.f + z);
+}
 __device__ __forceinline__ float sigmoid_f32(float l) {
     const float z = expf(-fabsf(l));
     return (l >= 0.f ? 1.f : z) / (1.f + z);
 }
 
-// Softmax statistics of the row: exact maximum, sum in 32 and (on demand) 64 bits.
+// Softmax statistics of the row: exact maximum, sum in 32 bits.
 struct RowStats {
     float top, sum;
-    double sum64;
-    bool has64;
 };
 
-template <int kPerLane>
-__device__ __noinline__ double row_sum_f64(const RouteParams& p, uint64_t row, uint32_t first, uint32_t n, float top) {
+template <typename T>
+__device__ double row_sum_f64(const RouteParams& p, uint64_t row, uint32_t first, uint32_t n, float top) {
     double sum = 0.0;
     for (uint32_t i = 0; i < n; ++i) {
         float l, b;
-        if (load_logit(p, row, first + i, l, b)) sum += exp(double(l) - double(top));
+        if (load_logit<T>(p, row, first + i, l, b)) sum += exp(double(l) - double(top));
     }
-#pragma unroll
+#pragma unroll 1
     for (uint32_t d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     return sum;
 }
 
 // The score plus bias in 64 bits.
-__device__ __forceinline__ double key_f64(const RouteParams& p, const RowStats& s, float l, float b) {
+__device__ __forceinline__ double key_f64(const RouteParams& p, float top, double sum, float l, float b) {
     if (p.sigmoid) return 1.0 / (1.0 + exp(-double(l))) + double(b);
-    return exp(double(l) - double(s.top)) / s.sum64 + double(b);
+    return exp(double(l) - double(top)) / sum + double(b);
 }
 
-template <int kPerLane>
-__global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RouteParams p) {
+// Rank of this lane's group by f64 values (scores: sums of two or the largest).
+template <typename T>
+__device__ __noinline__ uint32_t group_rank_f64(const RouteParams& p, uint64_t row, uint32_t first, uint32_t n, uint32_t group,
+                                                float top, bool by_sum) {
     constexpr uint32_t kAll = 0xffffffffu;
+    const bool scored = p.bias != nullptr || by_sum;
+    const double sum = scored && !p.sigmoid ? row_sum_f64<T>(p, row, first, n, top) : 1.0;
+    double b1 = -INFINITY, b2 = -INFINITY;
+    for (uint32_t i = 0; i < n; ++i) {
+        float l, b;
+        if (!load_logit<T>(p, row, first + i, l, b)) continue;
+        const double m = scored ? key_f64(p, top, sum, l, b) : double(l);
+        b2 = fmax(b2, fmin(b1, m));
+        b1 = fmax(b1, m);
+    }
+    for (uint32_t d = (1u << p.lanes_log2) >> 1; d > 0; d >>= 1) {
+        const double o1 = __shfl_xor_sync(kAll, b1, d), o2 = __shfl_xor_sync(kAll, b2, d);
+        b2 = fmax(fmin(b1, o1), fmax(b2, o2));
+        b1 = fmax(b1, o1);
+    }
+    const double mine = by_sum && b2 > -INFINITY ? b1 + b2 : b1;
+    uint32_t rank = 0;
+    for (uint32_t o = 0; o < p.num_groups; ++o) {
+        const double v = __shfl_sync(kAll, mine, o << p.lanes_log2);
+        rank += v > mine || (v == mine && o < group);
+    }
+    return rank;
+}
+
+// The row's choices by f64 keys (the logits themselves without a bias): lane j returns the
+// j-th expert, or -1.
+template <typename T>
+__device__ __noinline__ int choose_f64(const RouteParams& p, uint64_t row, uint32_t first, uint32_t n, bool eligible, float top) {
+    constexpr uint32_t kAll = 0xffffffffu;
+    const bool keyed = p.bias != nullptr;
+    const double sum = keyed && !p.sigmoid ? row_sum_f64<T>(p, row, first, n, top) : 1.0;
+    uint64_t key[kRouteMaxPerLane];
+    for (uint32_t i = 0; i < n; ++i) {
+        float l, b;
+        const bool alive = load_logit<T>(p, row, first + i, l, b) && eligible;
+        key[i] = !alive ? 0 : order_f64(keyed ? key_f64(p, top, sum, l, b) : double(l));
+    }
+    int chosen = -1;
+    for (uint32_t j = 0; j < p.topk; ++j) {
+        uint64_t best = 0;
+        uint32_t at = 0;
+        for (uint32_t i = 0; i < n; ++i)
+            if (key[i] > best) { best = key[i]; at = i; }              // equal keys: the first
+        const uint32_t high = uint32_t(best >> 32), low = uint32_t(best);
+        const uint32_t top_high = __reduce_max_sync(kAll, high);
+        if (top_high == 0) break;                                      // no float orders below 2^32
+        const uint32_t top_low = __reduce_max_sync(kAll, high == top_high ? low : 0u);
+        const uint32_t winner = __ffs(__ballot_sync(kAll, high == top_high && low == top_low)) - 1;
+        const uint32_t e = __shfl_sync(kAll, first + at, winner);
+        if (threadIdx.x % 32 == j) chosen = int(e);
+        if (threadIdx.x % 32 == winner) key[at] = 0;
+    }
+    return chosen;
+}
+
+// Batcher's odd-even merge sort of a lane's list, largest first.
+template <int kCount>
+__device__ __forceinline__ void sort_descending(uint32_t (&v)[kCount]) {
+#pragma unroll
+    for (int p = 1; p < kCount; p *= 2)
+#pragma unroll
+        for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+            for (int i = 0; i + k < kCount; ++i)
+                if (i >= k % p && (i - k % p) / k % 2 == 0 && i / (2 * p) == (i + k) / (2 * p)) {
+                    const uint32_t x = v[i], y = v[i + k];
+                    v[i] = max(x, y);
+                    v[i + k] = min(x, y);
+                }
+}
+
+// Whether the order of two neighbours is in doubt: keys a >= b, of which the lowest bits
+// (`mask`) are not the float's, each off by at most `error` and the rounding of a sum, 2^-24
+// of its size (the difference taken here rounds once more).
+__device__ __forceinline__ bool in_doubt(uint32_t a, uint32_t b, uint32_t mask, float error) {
+    const float low = unorder_f32(a & ~mask), high = unorder_f32(b | mask);
+    return b != 0 && !(low - high > 2.f * error + 0x1p-22f * fmaxf(fabsf(low), fabsf(high)));   // NaN: in doubt
+}
+
+// kFull: every lane of a group has kPerLane experts, in rows aligned for vector loads.
+template <typename T, int kPerLane, bool kFull>
+__global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_constant__ RouteParams p) {
+    constexpr uint32_t kAll = 0xffffffffu;
+    constexpr bool kSorted = kPerLane <= 16;
+    constexpr uint32_t kPlace = kPerLane - 1u;        // bits of a key that hold the place; kPerLane is a power of two
     const uint32_t lane = threadIdx.x & 31;
     const uint32_t t = blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
     ptx::launch_dependents();
@@ -115,203 +241,169 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RoutePara
     if (t >= p.num_tokens) return;                    // whole warps
 
     const uint64_t row = t * p.logits_stride;
-    const uint32_t group = lane / p.lanes_per_group, sub = lane % p.lanes_per_group;
+    const uint32_t group = lane >> p.lanes_log2, sub = lane & ((1u << p.lanes_log2) - 1u);
     const uint32_t begin = sub * p.per_lane;
     const uint32_t n = group < p.num_groups && begin < p.group_size ? min(p.per_lane, p.group_size - begin) : 0u;
     const uint32_t first = group * p.group_size + begin;
-    const bool has_bias = p.bias != nullptr;
+    const bool keyed = p.bias != nullptr;             // keys are scores, not logits
 
-    float value[kPerLane];                            // logits, then keys; -inf: not eligible
-    float bias[kPerLane];
-    float top = -INFINITY;
+    // Logits, then keys.  -inf or NaN: not eligible; a comparison with -inf tells both.
+    float value[kPerLane], bias[kPerLane];
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-        value[i] = -INFINITY;
-        bias[i] = 0.f;
-        if (uint32_t(i) < n) {
-            float l, b;
-            if (load_logit(p, row, first + i, l, b)) { value[i] = l; bias[i] = b; }
+    for (int i = 0; i < kPerLane; ++i) { value[i] = -INFINITY; bias[i] = 0.f; }
+    if constexpr (kFull) {
+        if (n != 0) {
+            load_run<kPerLane>(static_cast<const T*>(p.logits) + row + first, value);
+            if (keyed) load_run<kPerLane>(p.bias + first, bias);
         }
-        top = fmaxf(top, value[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kPerLane; ++i)
+            if (uint32_t(i) < n) {
+                value[i] = logit_f32(static_cast<const T*>(p.logits)[row + first + i]);
+                if (keyed) bias[i] = p.bias[first + i];
+            }
     }
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) value[i] = clean_logit(value[i]);
 
     const bool by_sum = p.num_groups > 1 && !p.group_by_max;
-    RowStats stats = {0.f, 1.f, 1.0, false};
-    if (!p.sigmoid && (has_bias || by_sum || !p.renormalize)) {
+    RowStats stats = {0.f, 1.f};
+    if (!p.sigmoid && (keyed || by_sum || !p.renormalize)) {
         // masked experts have no part in the softmax; an empty row keeps top = 0
+        float top = -INFINITY;
 #pragma unroll
-        for (uint32_t d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, d));
+        for (int i = 0; i < kPerLane; ++i)
+            if (bias[i] > -INFINITY) top = fmaxf(top, value[i]);       // fmaxf passes over NaN
+        top = unorder_f32(__reduce_max_sync(kAll, order_f32(top)));
         if (top > -INFINITY) {
             float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < kPerLane; ++i) sum += expf(value[i] - top);
+            for (int i = 0; i < kPerLane; ++i)
+                if (value[i] > -INFINITY && bias[i] > -INFINITY) sum += expf(value[i] - top);
 #pragma unroll
             for (uint32_t d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(kAll, sum, d);
             stats.top = top;
             stats.sum = sum;
         }
     }
-    // Bound on the f32 error of a score: sigmoid, a few roundings of a value below one;
-    // softmax, the sum's roundings (2048 terms at most, pairwise over lanes) and the exponent's.
-    const float score_error = p.sigmoid ? 0x1p-21f : 0x1p-17f;
+    // Bound on the f32 error of a score.  Sigmoid, below one: the approximate exponential is
+    // off by 2 + 1.2 |l| steps of 2^-23, times s (1 - s) at most 0.65 steps; the sum and the
+    // reciprocal add 1.5: 2.15 steps.  Softmax, below inv_sum: the sum's roundings (2048 terms
+    // at most, 69 of them one after the other) and the exponential's, below 2^-17 of it.
     const float inv_sum = 1.f / stats.sum;
-    const bool keyed = has_bias;                      // keys are scores, not logits
-    auto score = [&](float l) { return p.sigmoid ? sigmoid_f32(l) : expf(l - stats.top) * inv_sum; };
-    auto need_sum64 = [&]() {
-        if (!p.sigmoid && !stats.has64) {
-            stats.sum64 = row_sum_f64<kPerLane>(p, row, first, n, stats.top);
-            stats.has64 = true;
-        }
-    };
+    const float score_error = p.sigmoid ? 0x1.2p-22f : 0x1p-17f * inv_sum;
+    // l * 0 makes the score of a masked logit NaN and leaves the others alone
+    auto score = [&](float l) { return fmaf(l, 0.f, p.sigmoid ? sigmoid_approx(l) : expf(l - stats.top) * inv_sum); };
+    if (keyed) {
+#pragma unroll
+        for (int i = 0; i < kPerLane; ++i) value[i] = score(value[i]) + bias[i];
+    }
+    constexpr bool kShort = sizeof(T) == 2;           // as f32, the low 13 bits of every logit are alike
 
     bool eligible = true;                             // this lane's group is among the best
     if (p.num_groups > 1) {
+        const bool scored = keyed || by_sum;          // the groups' values come from scores
         float a1 = -INFINITY, a2 = -INFINITY;         // the two largest members of the lane, then of the group
 #pragma unroll
         for (int i = 0; i < kPerLane; ++i) {
-            const bool alive = value[i] > -INFINITY;
-            const float m = !alive ? -INFINITY : (keyed || by_sum) ? score(value[i]) + bias[i] : value[i];
-            if (keyed) value[i] = m;
-            a2 = fmaxf(a2, fminf(a1, m));
+            const float m = !keyed && by_sum ? score(value[i]) : value[i];
+            a2 = fmaxf(a2, min_nan(a1, m));           // fmaxf passes over NaN
             a1 = fmaxf(a1, m);
         }
-        for (uint32_t d = p.lanes_per_group >> 1; d > 0; d >>= 1) {
+        for (uint32_t d = (1u << p.lanes_log2) >> 1; d > 0; d >>= 1) {
             const float o1 = __shfl_xor_sync(kAll, a1, d), o2 = __shfl_xor_sync(kAll, a2, d);
             a2 = fmaxf(fminf(a1, o1), fmaxf(a2, o2));
             a1 = fmaxf(a1, o1);
         }
         const bool two = by_sum && a2 > -INFINITY;
-        const float mine = two ? a1 + a2 : a1;
-        // a group without eligible experts has value -inf; bounds of the others' errors
-        float error = 0.f;
-        if ((keyed || by_sum) && mine > -INFINITY && mine < INFINITY)
-            error = (two ? 2.f : 1.f) * score_error + 0x1p-22f * (fabsf(a1) + (two ? fabsf(a2) : 0.f));
-        uint32_t rank = 0;
-        bool close = false;
-        for (uint32_t o = 0; o < p.num_groups; ++o) {
-            const float v = __shfl_sync(kAll, mine, o * p.lanes_per_group);
-            const float e = __shfl_sync(kAll, error, o * p.lanes_per_group);
-            rank += v > mine || (v == mine && o < group);
-            close |= o != group && fabsf(v - mine) <= e + error;
+        const float mine = two ? a1 + a2 : a1;        // -inf: nothing left in the group
+        // the group's place in the low bits; a group without members orders last, by place
+        const uint32_t packed = group < p.num_groups ? (order_f32(mine) & ~31u) | (31u - group) : 0u;
+        uint32_t left = packed, border = 0;
+        for (uint32_t r = 0; r < p.topk_groups; ++r) {
+            border = __reduce_max_sync(kAll, left);
+            if (left == border) left = 0;
         }
-        if ((keyed || by_sum) && __any_sync(kAll, close && group < p.num_groups)) {
-            need_sum64();
-            double b1 = -INFINITY, b2 = -INFINITY;
-            for (uint32_t i = 0; i < n; ++i) {
-                float l, b;
-                if (!load_logit(p, row, first + i, l, b)) continue;
-                const double m = key_f64(p, stats, l, b);
-                b2 = fmax(b2, fmin(b1, m));
-                b1 = fmax(b1, m);
-            }
-            for (uint32_t d = p.lanes_per_group >> 1; d > 0; d >>= 1) {
-                const double o1 = __shfl_xor_sync(kAll, b1, d), o2 = __shfl_xor_sync(kAll, b2, d);
-                b2 = fmax(fmin(b1, o1), fmax(b2, o2));
-                b1 = fmax(b1, o1);
-            }
-            const double exact = by_sum && b2 > -INFINITY ? b1 + b2 : b1;
-            rank = 0;
-            for (uint32_t o = 0; o < p.num_groups; ++o) {
-                const double v = __shfl_sync(kAll, exact, o * p.lanes_per_group);
-                rank += v > exact || (v == exact && o < group);
-            }
+        const uint32_t next = __reduce_max_sync(kAll, left);
+        eligible = packed >= border;
+        const bool empty = group < p.num_groups && mine == -INFINITY;
+        bool doubt = (border ^ next) < 32u && !(kShort && !scored);    // alike but for the place
+        if (scored) {
+            const float size = fabsf(mine) < INFINITY ? fabsf(a1) + (two ? fabsf(a2) : 0.f) : 0.f;
+            const float error = 2.f * score_error + 0x1p-22f * __uint_as_float(__reduce_max_sync(kAll, __float_as_uint(size)));
+            doubt = in_doubt(border, next, 31u, error);
         }
-        eligible = rank < p.topk_groups;
-    } else if (keyed) {
-#pragma unroll
-        for (int i = 0; i < kPerLane; ++i)
-            if (value[i] > -INFINITY) value[i] = score(value[i]) + bias[i];
+        // among groups without members the place decides: nothing is in doubt
+        if (doubt && !(__all_sync(kAll, left == 0 || empty)))
+            eligible = group_rank_f64<T>(p, row, first, n, group, stats.top, by_sum) < p.topk_groups;
     }
 
-    uint32_t key[kPerLane];
+    uint32_t list[kPerLane];
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) key[i] = eligible && value[i] > -INFINITY ? order_f32(value[i]) : 0u;
-
-    uint32_t best = 0, second = 0, best_i = 0;        // this lane's two largest keys
-    auto rescan = [&]() {
-        best = second = best_i = 0;
+    for (int i = 0; i < kPerLane; ++i)
+        list[i] = eligible && value[i] > -INFINITY ? (order_f32(value[i]) & ~kPlace) | (kPlace - uint32_t(i)) : 0u;
+    if constexpr (kSorted) sort_descending(list);
+    uint32_t mine = 0, owner = 0, last = 0;           // lane j: the j-th choice and its lane; the best that is left
+    for (uint32_t j = 0; j <= p.topk; ++j) {
+        uint32_t best = list[0];
+        if constexpr (!kSorted) {
 #pragma unroll
-        for (int i = 0; i < kPerLane; ++i) {
-            const bool up = key[i] > best;            // equal keys: the first stays
-            second = max(second, up ? best : key[i]);
-            best_i = up ? i : best_i;
-            best = up ? key[i] : best;
+            for (int i = 1; i < kPerLane; ++i) best = max(best, list[i]);
         }
-    };
-    rescan();
-    int chosen = -1;                                  // lane j: the j-th choice
-    for (uint32_t j = 0; j < p.topk; ++j) {
-        const uint32_t m = __reduce_max_sync(kAll, best);
-        if (m == 0) break;
-        uint32_t winner;
-        if (!keyed) {
-            winner = __ffs(__ballot_sync(kAll, best == m)) - 1;
+        // without the places: of equal keys the lower lane has the lower expert
+        const uint32_t m = __reduce_max_sync(kAll, best | kPlace);
+        if (m == kPlace) break;
+        if (j == p.topk) { last = m; break; }
+        const uint32_t winner = __ffs(__ballot_sync(kAll, (best | kPlace) == m)) - 1;
+        const uint32_t key = __shfl_sync(kAll, best, winner);
+        if (lane == j) { mine = key; owner = winner; }
+        const bool won = lane == winner;
+        if constexpr (kSorted) {
+#pragma unroll
+            for (int i = 0; i + 1 < kPerLane; ++i) list[i] = won ? list[i + 1] : list[i];
+            list[kPerLane - 1] = won ? 0u : list[kPerLane - 1];
         } else {
-            const float mf = unorder_f32(m);
-            const uint32_t bar = fabsf(mf) < INFINITY ? order_f32(mf - 2.f * (score_error + 0x1p-22f * fabsf(mf))) : m;
-            const uint32_t near = __ballot_sync(kAll, best >= bar);
-            if (__popc(near) == 1 && !__any_sync(kAll, second >= bar)) {
-                winner = __ffs(near) - 1;
-            } else {
-                need_sum64();
-                uint64_t exact = 0;
-                uint32_t exact_i = 0;
-#pragma unroll 1
-                for (uint32_t i = 0; i < n; ++i) {
-                    uint32_t k = 0;
 #pragma unroll
-                    for (int s = 0; s < kPerLane; ++s) k = uint32_t(s) == i ? key[s] : k;
-                    if (k == 0 || k < bar) continue;
-                    float l, b;
-                    load_logit(p, row, first + i, l, b);
-                    const uint64_t o = order_f64(key_f64(p, stats, l, b));
-                    if (o > exact) { exact = o; exact_i = i; }
-                }
-                const uint32_t high = uint32_t(exact >> 32), low = uint32_t(exact);
-                const uint32_t top_high = __reduce_max_sync(kAll, high);
-                const uint32_t top_low = __reduce_max_sync(kAll, high == top_high ? low : 0u);
-                winner = __ffs(__ballot_sync(kAll, exact != 0 && high == top_high && low == top_low)) - 1;
-                if (lane == winner) best_i = exact_i;
-            }
+            for (int i = 0; i < kPerLane; ++i) list[i] = won && list[i] == key ? 0u : list[i];
         }
-        const uint32_t e = __shfl_sync(kAll, first + best_i, winner);
-        if (lane == j) chosen = int(e);
-        if (lane == winner) {
-#pragma unroll
-            for (int i = 0; i < kPerLane; ++i) key[i] = uint32_t(i) == best_i ? 0u : key[i];
-            rescan();
-        }
+    }
+    const uint32_t after = __shfl_down_sync(kAll, mine, 1);
+    const uint32_t next = lane + 1 == p.topk ? last : after;
+    bool doubt = false;
+    if (lane < p.topk && mine != 0)
+        doubt = keyed ? in_doubt(mine, next, kPlace, score_error) : !kShort && (mine ^ next) <= kPlace;
+    int chosen = -1;
+    if (__any_sync(kAll, doubt)) {
+        chosen = choose_f64<T>(p, row, first, n, eligible, stats.top);
+    } else if (mine != 0) {
+        chosen = int((owner >> p.lanes_log2) * p.group_size + (owner & ((1u << p.lanes_log2) - 1u)) * p.per_lane + kPlace -
+                     (mine & kPlace));
     }
 
     // Weights: lane j has the j-th choice.  Renormalised scores are ratios, so they are
     // taken relative to the largest chosen one and no sum underflows:
     // sigmoid(l) = e^l / (1 + e^l) = e^m * (e^(l-m) / (1 + e^l)), m = min(0, largest l).
     float l = -INFINITY;
-    if (chosen >= 0) {
-        float b;
-        load_logit(p, row, chosen, l, b);
-    }
+    if (chosen >= 0) l = clean_logit(logit_f32(static_cast<const T*>(p.logits)[row + chosen]));
     float weight = 0.f;
     if (p.renormalize) {
-        float peak = l;
-#pragma unroll
-        for (uint32_t d = 16; d > 0; d >>= 1) peak = fmaxf(peak, __shfl_xor_sync(kAll, peak, d));
+        const float peak = unorder_f32(__reduce_max_sync(kAll, order_f32(l)));
         if (chosen >= 0) {
-            if (!p.sigmoid) weight = expf(l - peak);
-            else if (l > 0.f) weight = 1.f / (1.f + expf(-l));
-            else weight = expf(l - fminf(peak, 0.f)) / (1.f + expf(l));
+            weight = p.sigmoid && l > 0.f ? 1.f : expf(l - (p.sigmoid ? fminf(peak, 0.f) : peak));
+            if (p.sigmoid) weight /= 1.f + expf(-fabsf(l));
         }
         float sum = weight;
 #pragma unroll
         for (uint32_t d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(kAll, sum, d);
         if (chosen >= 0) weight /= sum;
     } else if (chosen >= 0) {
-        weight = score(l);
+        weight = p.sigmoid ? sigmoid_f32(l) : expf(l - stats.top) / stats.sum;
     }
     if (lane < p.topk) {
-        const uint64_t at = static_cast<uint64_t>(t) * p.topk + lane;
-        p.topk_idx[at] = chosen;
-        p.topk_weights[at] = weight * p.scale;
+        const uint64_t out = static_cast<uint64_t>(t) * p.topk + lane;
+        p.topk_idx[out] = chosen;
+        p.topk_weights[out] = weight * p.scale;
     }
 }
 

@@ -105,8 +105,13 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_fma_kernel(const Logits
 // kChainBlocks K blocks (512 channels: 4.7e-7) and its accumulator is added to f32 sums in
 // registers, rounded to nearest; two accumulators in TMEM keep the MMAs going meanwhile.
 //
-// Warp 0: TMA loads; warp 1: MMAs; warps 2-9: accumulators to registers, then the sums.
-constexpr uint32_t kLogitsMmaThreads = 320;
+// A TMA request costs its thread about 60 ns however small it is, so a stage holds several
+// K blocks, brought by one request per operand (a [K/64][rows][64] view of the rows, when H
+// is a multiple of 64) and issued by two warps.
+//
+// Warp 0: loads of x; warp 1: MMAs; warps 2-9: accumulators to registers, then the sums;
+// warp 10: loads of W.
+constexpr uint32_t kLogitsMmaThreads = 352;
 constexpr uint32_t kLogitsTileTokens = 128;
 constexpr uint32_t kLogitsBlockK = 64;
 constexpr uint32_t kChainBlocks = 8;
@@ -116,8 +121,10 @@ static __device__ uint32_t g_producer_status[kStatusWords];
 
 template <int kN>
 struct LogitsTile {
-    static constexpr uint32_t kStageBytes = kLogitsTileTokens * 128 + kN * 128;
-    static constexpr uint32_t kStages = kN == 256 ? 4 : kN == 128 ? 6 : 8;
+    static constexpr uint32_t kStageBlocks = kN == 256 ? 1 : 2;           // K blocks of a stage
+    static constexpr uint32_t kStageBytes = kStageBlocks * (kLogitsTileTokens + kN) * 128;
+    static constexpr uint32_t kStages = kN == 128 ? 3 : 4;
+    static constexpr uint32_t kChainStages = kChainBlocks / kStageBlocks;
     static constexpr uint32_t kPitch = kN + 4;                 // floats per row of the partial tile: no bank conflicts
     static constexpr uint32_t kDataBytes = kStages * kStageBytes;
     static_assert(kDataBytes >= kLogitsTileTokens * kPitch * 4, "the partial tile reuses the stages");
@@ -127,33 +134,52 @@ struct LogitsTile {
 };
 
 struct LogitsMmaParams {
-    CUtensorMap x_map;            // bf16 [T][H], box 64 x 128, 128-byte swizzle
-    CUtensorMap w_map;            // bf16 [P * E][H], box 64 x kN
+    CUtensorMap x_map;            // bf16 [T][H], 128-byte swizzle: box 64 x box_tokens (x kStageBlocks)
+    CUtensorMap w_map;            // bf16 [P * E][H], box 64 x kN (x kStageBlocks)
     float* out;                   // [T][E]
     uint32_t num_tokens, num_experts;
-    uint32_t k_blocks, planes;    // ceil(H / 64); planes alternate inside a K block
+    uint32_t k_stages, planes;    // stages that cover H; the planes alternate stage by stage
+    uint32_t box_tokens;          // rows a load of x brings: fewer than a tile when there are fewer tokens; the rest of
+                                  // the tile's rows keep what shared memory held and end in rows that are not stored
+    uint32_t wide;                // 1: maps are [K/64][rows][64] views, one request per operand and stage
     uint32_t split;               // CTAs of a cluster
 };
+
+// One operand of a stage: `rows` rows from `row` on, K blocks from `block` on.  Blocks past H
+// are filled with zeros.
+template <int kBlocks>
+__device__ __forceinline__ void load_operand(const CUtensorMap* map, uint32_t wide, uint32_t dst, uint32_t bar, uint32_t rows,
+                                             uint32_t row, uint32_t block, uint64_t hint) {
+    ptx::mbar_arrive_expect_tx(bar, kBlocks * rows * 128);
+    if (wide) {
+        ptx::tma_load_3d(dst, map, bar, 0, int(row), int(block), hint);
+    } else {
+#pragma unroll
+        for (uint32_t j = 0; j < kBlocks; ++j)
+            ptx::tma_load_2d(dst + j * rows * 128, map, bar, int((block + j) * kLogitsBlockK), int(row), hint);
+    }
+}
 
 template <int kN>
 __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const __grid_constant__ LogitsMmaParams p) {
     using Tile = LogitsTile<kN>;
+    constexpr uint32_t kBlocks = Tile::kStageBlocks, kStages = Tile::kStages;
     extern __shared__ uint8_t raw_smem[];
     const uint32_t base = (ptx::smem_u32(raw_smem) + 1023u) & ~1023u;     // swizzle atoms start on 1 KiB
     uint8_t* const smem = raw_smem + (base - ptx::smem_u32(raw_smem));
     const uint32_t bars = base + Tile::kDataBytes;
-    const uint32_t bar_full = bars, bar_empty = bars + 8 * Tile::kStages, bar_acc_full = bars + 16 * Tile::kStages;
+    const uint32_t bar_full = bars, bar_empty = bars + 8 * kStages, bar_acc_full = bars + 16 * kStages;
     const uint32_t bar_acc_empty = bar_acc_full + 16, bar_drain = bar_acc_full + 32;
-    volatile uint32_t* const tmem_slot =
-        reinterpret_cast<volatile uint32_t*>(smem + Tile::kDataBytes + (2 * Tile::kStages + 5) * 8);
+    volatile uint32_t* const tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + Tile::kDataBytes + (2 * kStages + 5) * 8);
     volatile uint32_t* const abort_word = tmem_slot + 1;
 
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = blockIdx.x;                                     // of the cluster: the K range
     const uint32_t e0 = blockIdx.y * kN, t0 = blockIdx.z * kLogitsTileTokens;
-    const uint32_t blocks = p.k_blocks * p.planes;
-    const uint32_t first = uint32_t(uint64_t(blocks) * rank / p.split);
-    const uint32_t count = uint32_t(uint64_t(blocks) * (rank + 1) / p.split) - first;   // >= 1: split <= blocks
+    const uint32_t steps = p.k_stages * p.planes;
+    const uint32_t first = uint32_t(uint64_t(steps) * rank / p.split);
+    const uint32_t count = uint32_t(uint64_t(steps) * (rank + 1) / p.split) - first;   // >= 1: split <= steps
+    const uint32_t x_bytes = kBlocks * p.box_tokens * 128;                // W follows x in a stage, on a 1 KiB boundary
 
     WaitCtl ctl;
     ctl.status = g_producer_status;
@@ -165,8 +191,8 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
     if (tid == 0) {
         ptx::prefetch_tensormap(&p.x_map);
         ptx::prefetch_tensormap(&p.w_map);
-        for (uint32_t i = 0; i < Tile::kStages; ++i) {
-            ptx::mbar_init(bar_full + 8 * i, 1);
+        for (uint32_t i = 0; i < kStages; ++i) {
+            ptx::mbar_init(bar_full + 8 * i, 2);
             ptx::mbar_init(bar_empty + 8 * i, 1);
         }
         for (uint32_t i = 0; i < 2; ++i) {
@@ -190,25 +216,27 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
     const uint32_t tmem = *tmem_slot;
 
     float acc[kN / 2];                                                    // warps 2-9: one token, half of the experts
-    if (warp == 0) {
+    if (warp == 0 || warp == 10) {
         if (ptx::elect_one()) {
-            uint32_t i = 0;
+            // Counters instead of divisions: the loop is a chain of one thread's instructions.
+            uint32_t ks = first / p.planes, plane = first - ks * p.planes;
+            uint32_t i = 0, stage = 0, parity = 1;                        // the first round finds the stages empty
             for (; i < count; ++i) {
-                const uint32_t stage = i % Tile::kStages, round = i / Tile::kStages;
-                if (round > 0 && !mbar_wait(bar_empty + 8 * stage, (round - 1) & 1, ctl, 1)) break;
-                const uint32_t block = first + i, kb = block / p.planes, plane = block - kb * p.planes;
-                const uint32_t a = base + stage * Tile::kStageBytes, b = a + kLogitsTileTokens * 128;
-                ptx::mbar_arrive_expect_tx(bar_full + 8 * stage, Tile::kStageBytes);
-                ptx::tma_load_2d(a, &p.x_map, bar_full + 8 * stage, int(kb * kLogitsBlockK), int(t0), ptx::kEvictNormal);
-                ptx::tma_load_2d(b, &p.w_map, bar_full + 8 * stage, int(kb * kLogitsBlockK),
-                                 int(plane * p.num_experts + e0), ptx::kEvictLast);
+                if (i >= kStages && !mbar_wait(bar_empty + 8 * stage, parity, ctl, 1)) break;
+                const uint32_t dst = base + stage * Tile::kStageBytes, bar = bar_full + 8 * stage;
+                if (warp == 0)
+                    load_operand<kBlocks>(&p.x_map, p.wide, dst, bar, p.box_tokens, t0, ks * kBlocks, ptx::kEvictNormal);
+                else
+                    load_operand<kBlocks>(&p.w_map, p.wide, dst + x_bytes, bar, kN, plane * p.num_experts + e0, ks * kBlocks,
+                                          ptx::kEvictLast);
+                if (++plane == p.planes) { plane = 0; ++ks; }
+                if (++stage == kStages) { stage = 0; parity ^= 1; }
             }
             if (i < count) {
-                // Gave up: the copies in flight land before shared memory is used again.
+                // Gave up: the copies in flight land (or have time to) before shared memory is used again.
                 const uint64_t start = ptx::globaltimer_ns();
-                const uint32_t oldest = i > Tile::kStages ? i - Tile::kStages : 0;
-                for (uint32_t j = oldest; j < i; ++j)
-                    while (!ptx::mbar_try_wait(bar_full + 8 * (j % Tile::kStages), (j / Tile::kStages) & 1) &&
+                for (uint32_t j = i > kStages ? i - kStages : 0; j < i; ++j)
+                    while (!ptx::mbar_try_wait(bar_full + 8 * (j % kStages), (j / kStages) & 1) &&
                            ptx::globaltimer_ns() - start < 2000000ull) {}
             }
         }
@@ -216,17 +244,26 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
     } else if (warp == 1) {
         if (ptx::elect_one()) {
             constexpr uint32_t idesc = ptx::instr_desc_bf16(kLogitsTileTokens, kN);
-            uint32_t i = 0;
+            const uint64_t a_desc = ptx::smem_desc(base, 1024, true), b_desc = ptx::smem_desc(base + x_bytes, 1024, true);
+            const uint32_t a_block = p.box_tokens * 128 >> 4;             // descriptors count 16-byte units
+            uint32_t i = 0, stage = 0, parity = 0, chain = 0, step = 0;
             for (; i < count; ++i) {
-                const uint32_t stage = i % Tile::kStages, chain = i / kChainBlocks, step = i % kChainBlocks;
-                if (step == 0 && chain >= 2 && !mbar_wait(bar_acc_empty + 8 * (chain & 1), ((chain >> 1) - 1) & 1, ctl, 2)) break;
-                if (!mbar_wait(bar_full + 8 * stage, (i / Tile::kStages) & 1, ctl, 3)) break;
+                const uint32_t which = chain & 1;
+                if (step == 0 && chain >= 2 && !mbar_wait(bar_acc_empty + 8 * which, ((chain >> 1) - 1) & 1, ctl, 2)) break;
+                if (!mbar_wait(bar_full + 8 * stage, parity, ctl, 3)) break;
                 ptx::tc_fence_after();
-                const uint32_t a = base + stage * Tile::kStageBytes, b = a + kLogitsTileTokens * 128;
-                ptx::mma_bf16_k64(tmem + (chain & 1) * kN, ptx::smem_desc(a, 1024, true), ptx::smem_desc(b, 1024, true), idesc,
-                                  step != 0);
+                const uint32_t at = stage * (Tile::kStageBytes >> 4);
+#pragma unroll
+                for (uint32_t j = 0; j < kBlocks; ++j)
+                    ptx::mma_bf16_k64(tmem + which * kN, a_desc + at + j * a_block, b_desc + at + j * (kN * 128 >> 4), idesc,
+                                      step + j != 0);
                 ptx::tc_commit<false>(bar_empty + 8 * stage);
-                if (step == kChainBlocks - 1 || i == count - 1) ptx::tc_commit<false>(bar_acc_full + 8 * (chain & 1));
+                if (++step == Tile::kChainStages || i == count - 1) {
+                    ptx::tc_commit<false>(bar_acc_full + 8 * which);
+                    step = 0;
+                    ++chain;
+                }
+                if (++stage == kStages) { stage = 0; parity ^= 1; }
             }
             if (i < count) {
                 // Gave up: the MMAs in flight end before TMEM is freed and shared memory reused.
@@ -239,7 +276,7 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
     } else {
         const uint32_t half = (warp - 2) >> 2;
         const uint32_t lanes = (warp & 3) << 21;                          // this warp's quarter of the TMEM lanes
-        const uint32_t chains = (count + kChainBlocks - 1) / kChainBlocks;
+        const uint32_t chains = (count + Tile::kChainStages - 1) / Tile::kChainStages;
 #pragma unroll
         for (int j = 0; j < kN / 2; ++j) acc[j] = 0.f;
         for (uint32_t chain = 0; chain < chains; ++chain) {
@@ -264,7 +301,7 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
     __syncthreads();
     // The partial tile replaces the stages: every load has been consumed and every MMA has
     // ended (the last chain's barrier), or has been drained above.
-    if (warp >= 2) {
+    if (warp >= 2 && warp < 10) {
         const bool failed = *abort_word != 0u;
         const uint32_t half = (warp - 2) >> 2, token = (warp & 3) * 32 + lane;
         float4* const row = reinterpret_cast<float4*>(smem + (token * Tile::kPitch + half * (kN / 2)) * 4);
@@ -280,6 +317,7 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
         if (e0 + c >= p.num_experts) continue;
         const uint32_t at = base + (r * Tile::kPitch + c) * 4;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+
         for (uint32_t s = 0; s < p.split; ++s) {
             const float4 v = ptx::ld_cluster_f32x4(ptx::mapa(at, s));
             sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;

@@ -38,6 +38,11 @@ def _row_stride(t: torch.Tensor, hidden: int) -> int:
     return t.stride(0) if t.shape[0] > 1 else hidden
 
 
+def _rows_like(t: torch.Tensor) -> torch.Tensor:
+    """New contiguous tensor of the shape and type of ``t``."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def rms_norm_for_gc_moe(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None,
                         eps: float = 1e-6, *, normed: Union[bool, torch.Tensor] = True,
                         residual_out: Optional[torch.Tensor] = None, sym_buffer=None) -> NormedInputs:
@@ -69,7 +74,7 @@ def rms_norm_for_gc_moe(x: torch.Tensor, weight: torch.Tensor, residual: Optiona
     if residual is not None:
         _check_rows(residual, 'residual', shape, _FLOATS, device)
         if residual_out is None:
-            residual_out = torch.empty(shape, dtype=residual.dtype, device=residual.device)
+            residual_out = _rows_like(residual)
         elif residual_out is not residual:
             _check_rows(residual_out, 'residual_out', shape, (residual.dtype,), device)
         residual_ptr, residual_stride = residual.data_ptr(), _row_stride(residual, hidden)
@@ -78,15 +83,16 @@ def rms_norm_for_gc_moe(x: torch.Tensor, weight: torch.Tensor, residual: Optiona
     elif residual_out is not None:
         raise ValueError('residual_out needs a residual')
     if normed is True:
-        normed = torch.empty(shape, dtype=torch.bfloat16, device=x.device)
+        normed = _rows_like(x)
     elif normed is False or normed is None:
         normed = None
     else:
         _check_rows(normed, 'normed', shape, (torch.bfloat16,), device)
     shared_sf, shared_rows, block_m = None, 0, 0
     if sym_buffer is None:
-        x_q = torch.empty(shape, dtype=torch.float8_e4m3fn, device=x.device)
-        x_sf = torch.empty((tokens, (hidden + 127) // 128), dtype=torch.int32, device=x.device)
+        words = (hidden + 127) // 128
+        x_q = torch.empty_strided(shape, (hidden, 1), dtype=torch.float8_e4m3fn, device=x.device)
+        x_sf = torch.empty_strided((tokens, words), (words, 1), dtype=torch.int32, device=x.device)
     else:
         if sym_buffer.buffer is None:
             raise ValueError('symmetric buffer has been destroyed')
@@ -108,7 +114,7 @@ def rms_norm_for_gc_moe(x: torch.Tensor, weight: torch.Tensor, residual: Optiona
         _row_stride(x, hidden), residual_stride, 0 if normed is None else _row_stride(normed, hidden),
         residual_out_stride, shared_rows, block_m, tokens, hidden, residual_f32,
         int(weight.dtype is torch.float32), eps, device)
-    code = _native.library().gcmoe_rms_norm(ctypes.byref(args), torch.cuda.current_stream(device).cuda_stream)
+    code = _native.library().gcmoe_rms_norm(ctypes.byref(args), _native.current_stream(device))
     if code:
         _native.raise_for(code)
     return NormedInputs(x_q, x_sf, normed, residual_out)

@@ -72,13 +72,13 @@ def router_logits_for_gc_moe(x: torch.Tensor, router_weight: torch.Tensor,
     check_router_weight(router_weight, hidden, device)
     planes, experts = router_weight.shape[:2]
     if out is None:
-        out = torch.empty((tokens, experts), dtype=torch.float32, device=x.device)
+        out = torch.empty_strided((tokens, experts), (experts, 1), dtype=torch.float32, device=x.device)
     elif (out.shape != (tokens, experts) or out.dtype != torch.float32 or out.get_device() != device
           or not out.is_contiguous()):
         raise ValueError(f'out must be contiguous float32 [{tokens}, {experts}] on the device of x')
     args = _native.LogitsArgs(x.data_ptr(), router_weight.data_ptr(), out.data_ptr(),
                               x.stride(0) if tokens > 1 else hidden, tokens, hidden, experts, planes, device, 0)
-    code = _native.library().gcmoe_router_logits(ctypes.byref(args), torch.cuda.current_stream(device).cuda_stream)
+    code = _native.library().gcmoe_router_logits(ctypes.byref(args), _native.current_stream(device))
     if code:
         _native.raise_for(code)
     return out
@@ -140,8 +140,8 @@ def route_for_gc_moe(logits: torch.Tensor, topk: int, *, scoring: str = 'softmax
         topk_groups = num_groups
     check_routing(experts, topk, scoring, bias, num_groups, topk_groups, group_score, scale, device)
     if out is None:
-        idx = torch.empty((tokens, topk), dtype=torch.int64, device=logits.device)
-        weights = torch.empty((tokens, topk), dtype=torch.float32, device=logits.device)
+        idx = torch.empty_strided((tokens, topk), (topk, 1), dtype=torch.int64, device=logits.device)
+        weights = torch.empty_strided((tokens, topk), (topk, 1), dtype=torch.float32, device=logits.device)
     else:
         idx, weights = out
         for t, dtype in ((idx, torch.int64), (weights, torch.float32)):
@@ -152,7 +152,7 @@ def route_for_gc_moe(logits: torch.Tensor, topk: int, *, scoring: str = 'softmax
         logits.stride(0) if tokens > 1 else experts, tokens, experts, topk, num_groups, topk_groups,
         _LOGIT_TYPES[logits.dtype], _SCORINGS[scoring], _GROUP_SCORES[group_score], int(bool(renormalize)), scale,
         device, 0)
-    code = _native.library().gcmoe_route(ctypes.byref(args), torch.cuda.current_stream(device).cuda_stream)
+    code = _native.library().gcmoe_route(ctypes.byref(args), _native.current_stream(device))
     if code:
         _native.raise_for(code)
     return idx, weights
