@@ -792,7 +792,7 @@ extern "C" int gcmoe_rms_norm(const gcmoe_norm_args* args, void* cuda_stream) {
     p.x_stride = a.x_stride; p.residual_stride = a.residual_stride;
     p.normed_stride = a.normed_stride; p.residual_out_stride = a.residual_out_stride;
     p.shared_sf_rows = a.shared_sf_rows; p.block_m = a.block_m;
-    p.hidden = a.hidden; p.eps = a.eps; p.inv_hidden = 1.0f / float(a.hidden);
+    p.hidden = a.hidden; p.eps = a.eps;
     const uint32_t chunks = a.hidden / 8;
     uint32_t per_thread = 1;
     while (per_thread * kNormThreads < chunks) per_thread *= 2;
@@ -812,11 +812,10 @@ extern "C" int gcmoe_rms_norm(const gcmoe_norm_args* args, void* cuda_stream) {
     return GCMOE_OK;
 }
 
-template <int kPlanes>
+template <int kTokens, int kPlanes>
 static cudaError_t launch_logits_fma(const LogitsParams& p, cudaStream_t s) {
-    constexpr int kTokens = 4, kExperts = 2;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((p.num_experts + kExperts - 1) / kExperts, (p.num_tokens + kTokens - 1) / kTokens);
+    cfg.gridDim = dim3((p.num_experts + 1) / 2, (p.num_tokens + kTokens - 1) / kTokens);
     cfg.blockDim = dim3(kLogitsThreads);
     cfg.stream = s;
     cudaLaunchAttribute attr;
@@ -824,66 +823,65 @@ static cudaError_t launch_logits_fma(const LogitsParams& p, cudaStream_t s) {
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, logits_fma_kernel<kTokens, kExperts, kPlanes>, p);
+    return cudaLaunchKernelEx(&cfg, logits_fma_kernel<kTokens, kPlanes>, p);
 }
 
-// Experts per tile and CTAs per tile (the split of K) of the tensor-core form: the pair with
-// the least estimated time, in cycles.  A K block costs the bytes it brings from L2 or the
-// four MMAs, whichever is longer; a launch its waves over the SMs (clusters leave some SMs of
-// a GPC unused), a fixed start and end, and the partial tiles' way through shared memory.
+// Tile and split of the tensor-core form: the choice with the least estimated time, in
+// cycles.  A K block costs the bytes it brings from L2 (65 a cycle and SM with all SMs at it)
+// or its four MMAs, whichever is longer; a launch its waves over the SMs (clusters leave some
+// SMs of a GPC unused), a fixed start and end, and the partial tiles' way through shared
+// memory.  Over 24 sizes (1 to 4096 tokens, 64 to 384 experts, H 1056 to 7168, both weight
+// types) the choice was within 5% of the best of all tiles and splits, measured one by one:
+// 128 x 7168 x 256, for one, 6.2 us with 32 experts over 8 CTAs, 9.8 with 128 over 4;
+// 2048 x 7168 x 256 the other way round, 13.2 us with 128 over 4, 20 with 64 over 4.
 struct LogitsPlan {
     uint32_t experts, split;
 };
-static LogitsPlan plan_logits(uint32_t tokens, uint32_t experts, uint32_t blocks) {
+static LogitsPlan plan_logits(uint32_t tokens, uint32_t experts, uint32_t hidden, uint32_t planes) {
+    const uint64_t blocks = (hidden + kLogitsBlockK - 1) / kLogitsBlockK;
     const uint32_t rows = tokens < kLogitsTileTokens ? tokens : kLogitsTileTokens;
-    const uint64_t token_tiles = (tokens + kLogitsTileTokens - 1) / kLogitsTileTokens;
     LogitsPlan best = {32, 1};
     uint64_t least = ~0ull;
-    for (uint32_t n = 32; n <= 256; n *= 2) {
-        if (n > 32 && n / 2 >= experts) break;
-        for (uint32_t split = 1; split <= 16 && split <= blocks; split *= 2) {
-            const uint64_t ctas = token_tiles * ((experts + n - 1) / n) * split;
-            const uint64_t room = split >= 8 ? 128 : split == 4 ? 136 : 148;
+    for (uint32_t split = 1; split <= 8 && (split == 1 || split <= blocks / 2); split *= 2) {
+        for (uint32_t n = 32; n <= (planes == 1 ? 128u : 64u) && (n == 32 || n / 2 < experts); n *= 2) {
+            const uint32_t columns = n * planes;
+            const uint64_t ctas = uint64_t((tokens + kLogitsTileTokens - 1) / kLogitsTileTokens) * ((experts + n - 1) / n) * split;
+            const uint64_t room = split == 8 ? 112 : split == 4 ? 132 : 148;
             const uint64_t waves = (ctas + room - 1) / room, steps = (blocks + split - 1) / split;
-            const uint64_t bytes = (rows + n) * 128 / 48, mma = 2 * n;
-            const uint64_t time = waves * (steps * (bytes > mma ? bytes : mma) + 2000 + 10 * n + (split > 1 ? rows * n * 4 / 25 : 0));
+            const uint64_t bytes = (rows + columns) * 128 / 65;
+            const uint64_t mma = columns <= 96 ? 230 : columns == 128 ? 320 : 410;
+            const uint64_t time = waves * (steps * (bytes > mma ? bytes : mma) + 6500 + rows * n / 4);
             if (time < least) { least = time; best = {n, split}; }
         }
     }
     return best;
 }
 
-template <int kN>
+template <int kN, int kPlanes>
 static int launch_logits_mma(const gcmoe_logits_args& a, uint32_t split, cudaStream_t s) {
-    using Tile = LogitsTile<kN>;
+    using Tile = LogitsTile<kN, kPlanes>;
     LogitsMmaParams p;
     p.box_tokens = a.num_tokens < kLogitsTileTokens ? round_up_u32(a.num_tokens, 8) : kLogitsTileTokens;
-    p.wide = a.hidden % kLogitsBlockK == 0;
-    const uint64_t w_rows = uint64_t(a.planes) * a.num_experts, x_pitch = a.x_stride * 2, w_pitch = uint64_t(a.hidden) * 2;
-    const uint64_t k_blocks = a.hidden / kLogitsBlockK;
-    const uint64_t x_dims[3] = {p.wide ? kLogitsBlockK : a.hidden, a.num_tokens, k_blocks};
-    const uint64_t w_dims[3] = {p.wide ? kLogitsBlockK : a.hidden, w_rows, k_blocks};
-    const uint64_t x_strides[2] = {x_pitch, kLogitsBlockK * 2}, w_strides[2] = {w_pitch, kLogitsBlockK * 2};
-    const uint32_t x_box[3] = {kLogitsBlockK, p.box_tokens, Tile::kStageBlocks}, w_box[3] = {kLogitsBlockK, kN, Tile::kStageBlocks};
-    const uint32_t dims = p.wide ? 3 : 2;
-    if (int rc = encode_map(&p.x_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dims, a.x, x_dims, x_strides, x_box, "router input")) return rc;
-    if (int rc = encode_map(&p.w_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dims, a.weight, w_dims, w_strides, w_box, "router weight"))
+    const uint64_t x_dims[2] = {a.hidden, a.num_tokens}, w_dims[2] = {a.hidden, uint64_t(kPlanes) * a.num_experts};
+    const uint64_t x_pitch = a.x_stride * 2, w_pitch = uint64_t(a.hidden) * 2;
+    const uint32_t x_box[2] = {kLogitsBlockK, p.box_tokens}, w_box[2] = {kLogitsBlockK, kN};
+    if (int rc = encode_map(&p.x_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.x, x_dims, &x_pitch, x_box, "router input")) return rc;
+    if (int rc = encode_map(&p.w_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.weight, w_dims, &w_pitch, w_box, "router weight"))
         return rc;
     p.out = reinterpret_cast<float*>(a.out);
     p.num_tokens = a.num_tokens; p.num_experts = a.num_experts;
     p.k_stages = (a.hidden + kLogitsBlockK * Tile::kStageBlocks - 1) / (kLogitsBlockK * Tile::kStageBlocks);
-    p.planes = a.planes;
-    p.split = split < p.k_stages * p.planes ? split : p.k_stages * p.planes;
-    // the attribute is per device and outlives the call: set once for each
+    p.split = split;                                   // at most half of the K blocks: no CTA is without a stage
+    // the attributes are the device's and outlive the call: set once for each
     static std::atomic<uint64_t> ready{0};
     const uint64_t bit = 1ull << (a.device & 63);
     if (!(ready.load() & bit)) {
-        GCMOE_CUDA(cudaFuncSetAttribute(logits_mma_kernel<kN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile::kSmemBytes));
-        GCMOE_CUDA(cudaFuncSetAttribute(logits_mma_kernel<kN>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        GCMOE_CUDA(cudaFuncSetAttribute(logits_mma_kernel<kN, kPlanes>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        Tile::kSmemBytes));
         ready |= bit;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.split, (a.num_experts + kN - 1) / kN, (a.num_tokens + kLogitsTileTokens - 1) / kLogitsTileTokens);
+    cfg.gridDim = dim3(split, (a.num_experts + kN - 1) / kN, (a.num_tokens + kLogitsTileTokens - 1) / kLogitsTileTokens);
     cfg.blockDim = dim3(kLogitsMmaThreads);
     cfg.dynamicSmemBytes = Tile::kSmemBytes;
     cfg.stream = s;
@@ -891,11 +889,11 @@ static int launch_logits_mma(const gcmoe_logits_args& a, uint32_t split, cudaStr
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = p.split;
+    attr[1].val.clusterDim.x = split;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    GCMOE_CUDA(cudaLaunchKernelEx(&cfg, logits_mma_kernel<kN>, p));
+    GCMOE_CUDA(cudaLaunchKernelEx(&cfg, logits_mma_kernel<kN, kPlanes>, p));
     return GCMOE_OK;
 }
 
@@ -920,16 +918,23 @@ extern "C" int gcmoe_router_logits(const gcmoe_logits_args* args, void* cuda_str
     cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
     // Rows that overlap (a broadcast row) have no tensor map.
     if (a.num_tokens <= kFmaMaxTokens || a.x_stride < a.hidden || a.x_stride >= (1ull << 39)) {
-        GCMOE_CUDA(a.planes == 1 ? launch_logits_fma<1>(p, s) : launch_logits_fma<3>(p, s));
+        auto by_tokens = [&](auto planes) {
+            constexpr int kPlanes = decltype(planes)::value;
+            return p.num_tokens == 1   ? launch_logits_fma<1, kPlanes>(p, s)
+                   : p.num_tokens == 2 ? launch_logits_fma<2, kPlanes>(p, s)
+                                       : launch_logits_fma<4, kPlanes>(p, s);
+        };
+        GCMOE_CUDA(a.planes == 1 ? by_tokens(std::integral_constant<int, 1>()) : by_tokens(std::integral_constant<int, 3>()));
         return GCMOE_OK;
     }
-    const uint32_t blocks = (a.hidden + kLogitsBlockK - 1) / kLogitsBlockK * a.planes;
-    const LogitsPlan plan = plan_logits(a.num_tokens, a.num_experts, blocks);
+    const LogitsPlan plan = plan_logits(a.num_tokens, a.num_experts, a.hidden, a.planes);
+    if (a.planes == 3)
+        return plan.experts == 32 ? launch_logits_mma<32, 3>(a, plan.split, s)
+                                  : launch_logits_mma<64, 3>(a, plan.split, s);
     switch (plan.experts) {
-        case 32: return launch_logits_mma<32>(a, plan.split, s);
-        case 64: return launch_logits_mma<64>(a, plan.split, s);
-        case 128: return launch_logits_mma<128>(a, plan.split, s);
-        default: return launch_logits_mma<256>(a, plan.split, s);
+        case 32: return launch_logits_mma<32, 1>(a, plan.split, s);
+        case 64: return launch_logits_mma<64, 1>(a, plan.split, s);
+        default: return launch_logits_mma<128, 1>(a, plan.split, s);
     }
 }
 

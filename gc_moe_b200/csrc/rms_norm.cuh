@@ -41,7 +41,7 @@ struct NormParams {
     uint64_t x_stride, residual_stride, normed_stride, residual_out_stride;   // elements between rows
     uint32_t shared_sf_rows, block_m;
     uint32_t hidden;
-    float eps, inv_hidden;
+    float eps;
 };
 
 __device__ __forceinline__ void unpack_bf16x8(const uint4& raw, float (&v)[8]) {
@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(kNormThreads) rms_norm_kernel(const NormParams
 #pragma unroll
     for (uint32_t d = 8; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
     total = __shfl_sync(0xffffffffu, total, 0);
-    const float scale = 1.0f / sqrtf(total * p.inv_hidden + p.eps);
+    const float scale = 1.0f / sqrtf(total / float(p.hidden) + p.eps);
 
     uint32_t shared_row = 0;
     if (p.shared_sf != nullptr) {

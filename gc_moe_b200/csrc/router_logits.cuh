@@ -4,8 +4,7 @@
 // weight, three for an f32 weight (8 + 8 + 8 significant bits), so that every product is an
 // exact product of BF16 values and the result has the accuracy of f32 sums.
 //
-// A CTA takes kExperts experts and kTokens tokens; its threads run over K side by side and
-// their sums are added in a fixed order (no atomics, no dependence on the grid).
+// Sums are added in an order that the sizes fix: no atomics.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -28,11 +27,16 @@ struct LogitsParams {
     uint32_t num_tokens, num_experts, hidden;
 };
 
-constexpr uint32_t kFmaMaxTokens = 8;         // above: the tensor-core form
+// Few tokens: bound by the latency of the loads, so a thread has the loads of several
+// rounds of the loop in flight.  Measured (H 7168, E 256), us for 1, 4, 8 and 16 tokens:
+// BF16 weight 2.6, 3.8, 4.1, 5.2 in this form, 5.0, 5.2, 5.2, 5.3 on the tensor cores; FP32
+// weight 4.3, 4.3, 4.5, 8.0 and 5.4, 5.7, 5.7, 5.9.
+constexpr uint32_t kFmaMaxTokens = 8;
 
-template <int kTokens, int kExperts, int kPlanes>
-__global__ void __launch_bounds__(kLogitsThreads) logits_fma_kernel(const LogitsParams p) {
-    constexpr int kSums = kTokens * kExperts;
+template <int kTokens, int kPlanes>
+__global__ void __launch_bounds__(kLogitsThreads) logits_fma_kernel(const __grid_constant__ LogitsParams p) {
+    constexpr int kExperts = 2, kSums = kTokens * kExperts;
+    constexpr int kRounds = kPlanes == 1 ? 4 : 2;             // rounds of loads in flight
     __shared__ float partial[kLogitsThreads / 32][kSums];
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t e0 = blockIdx.x * kExperts, t0 = blockIdx.y * kTokens;
@@ -40,40 +44,52 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_fma_kernel(const Logits
     ptx::launch_dependents();
     ptx::grid_dependency_wait();
 
+    // rows past the last are the last row again: loaded, never stored
+    const uint4* x[kTokens];
+    const uint4* w[kExperts];
+#pragma unroll
+    for (int i = 0; i < kTokens; ++i)
+        x[i] = reinterpret_cast<const uint4*>(p.x + min(t0 + i, p.num_tokens - 1) * p.x_stride);
+#pragma unroll
+    for (int e = 0; e < kExperts; ++e)
+        w[e] = reinterpret_cast<const uint4*>(p.weight + uint64_t(min(e0 + e, p.num_experts - 1)) * p.hidden);
+    const uint64_t plane = uint64_t(p.num_experts) * chunks;
+
     float acc[kTokens][kExperts] = {};
-    for (uint32_t c = tid; c < chunks; c += kLogitsThreads) {
-        uint4 xr[kTokens];
+    for (uint32_t c0 = tid; c0 < chunks; c0 += kLogitsThreads * kRounds) {
+        uint4 xr[kRounds][kTokens], wr[kRounds][kExperts][kPlanes];
 #pragma unroll
-        for (int i = 0; i < kTokens; ++i) {
-            xr[i] = make_uint4(0, 0, 0, 0);
-            if (t0 + i < p.num_tokens) xr[i] = __ldg(reinterpret_cast<const uint4*>(p.x + (t0 + i) * p.x_stride) + c);
+        for (int r = 0; r < kRounds; ++r) {
+            const uint32_t c = c0 + r * kLogitsThreads;
+            const bool in = c < chunks;
+#pragma unroll
+            for (int i = 0; i < kTokens; ++i) xr[r][i] = in ? __ldg(x[i] + c) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < kExperts; ++e)
+#pragma unroll
+                for (int q = 0; q < kPlanes; ++q) wr[r][e][q] = in ? __ldg(w[e] + q * plane + c) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
-        for (int e = 0; e < kExperts; ++e) {
-            uint4 wr[kPlanes];
+        for (int r = 0; r < kRounds; ++r)
 #pragma unroll
-            for (int q = 0; q < kPlanes; ++q) {
-                wr[q] = make_uint4(0, 0, 0, 0);
-                if (e0 + e < p.num_experts)
-                    wr[q] = __ldg(reinterpret_cast<const uint4*>(p.weight + (uint64_t(q) * p.num_experts + e0 + e) * p.hidden) + c);
-            }
-            float w[8];
-            unpack_bf16x8(wr[0], w);
-            if constexpr (kPlanes == 3) {              // exact: the planes are the bits of one f32
-                float mid[8], low[8];
-                unpack_bf16x8(wr[1], mid);
-                unpack_bf16x8(wr[2], low);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) w[j] += mid[j] + low[j];
-            }
-#pragma unroll
-            for (int i = 0; i < kTokens; ++i) {
+            for (int e = 0; e < kExperts; ++e) {
                 float v[8];
-                unpack_bf16x8(xr[i], v);
+                unpack_bf16x8(wr[r][e][0], v);
+                if constexpr (kPlanes == 3) {              // exact: the planes are the bits of one f32
+                    float mid[8], low[8];
+                    unpack_bf16x8(wr[r][e][1], mid);
+                    unpack_bf16x8(wr[r][e][2], low);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) acc[i][e] = fmaf(v[j], w[j], acc[i][e]);
+                    for (int j = 0; j < 8; ++j) v[j] += mid[j] + low[j];
+                }
+#pragma unroll
+                for (int i = 0; i < kTokens; ++i) {
+                    float u[8];
+                    unpack_bf16x8(xr[r][i], u);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) acc[i][e] = fmaf(u[j], v[j], acc[i][e]);
+                }
             }
-        }
     }
 #pragma unroll
     for (int i = 0; i < kTokens; ++i)
@@ -89,15 +105,19 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_fma_kernel(const Logits
         const uint32_t t = t0 + tid / kExperts, e = e0 + tid % kExperts;
         float v = 0.f;
 #pragma unroll
-        for (uint32_t w = 0; w < kLogitsThreads / 32; ++w) v += partial[w][tid];
+        for (uint32_t g = 0; g < kLogitsThreads / 32; ++g) v += partial[g][tid];
         if (t < p.num_tokens && e < p.num_experts) p.out[static_cast<uint64_t>(t) * p.num_experts + e] = v;
     }
 }
 
 // ---------------------------------------------------------------------------------------
-// Tensor-core form, for more than a few tokens: 128 tokens x kN experts per tile, the K
-// blocks (64 channels of one weight plane) of a tile split over the CTAs of a cluster, whose
-// partial tiles are added through distributed shared memory in rank order.
+// Tensor-core form, for more than a few tokens: tiles of 128 tokens x kN experts, the K
+// blocks (64 channels) of a tile split over CTAs of a cluster, whose partial tiles are added
+// through distributed shared memory in rank order.
+//
+// The planes of an f32 weight are further columns of the tile's product: x is loaded once for
+// all three, and an MMA of 96 columns takes the time of one of 32 (the x operand's way out of
+// shared memory).  They are added to one sum when the accumulators are read.
 //
 // The tensor core truncates each addition to its f32 accumulator, always towards zero:
 // measured, the result of a K = 7168 product is 6.7e-6 too small in magnitude (relative
@@ -105,9 +125,12 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_fma_kernel(const Logits
 // kChainBlocks K blocks (512 channels: 4.7e-7) and its accumulator is added to f32 sums in
 // registers, rounded to nearest; two accumulators in TMEM keep the MMAs going meanwhile.
 //
-// A TMA request costs its thread about 60 ns however small it is, so a stage holds several
-// K blocks, brought by one request per operand (a [K/64][rows][64] view of the rows, when H
-// is a multiple of 64) and issued by two warps.
+// Bound by launch, TMA latency and the partial tiles' exchange for up to a few hundred tokens
+// (33 x 5120 x 384: 5.4 us), then by the traffic from L2 to the SMs: 4096 x 7168 x 256 takes
+// 20 us with 65 bytes a cycle and SM (235 MB in all; 10.2 us is what HBM needs for the inputs).
+// Tiles of 256 experts, as one CTA or as a pair with 256 tokens, move half to two thirds of
+// that but were no faster at any size: 20.8 and 22 us here, where their shared memory holds
+// too few stages to cover the latency.
 //
 // Warp 0: loads of x; warp 1: MMAs; warps 2-9: accumulators to registers, then the sums;
 // warp 10: loads of W.
@@ -119,50 +142,36 @@ constexpr uint32_t kChainBlocks = 8;
 // Where a wait of these launches gave up, for gcmoe_producer_status (they have no plan).
 static __device__ uint32_t g_producer_status[kStatusWords];
 
-template <int kN>
+template <int kN, int kPlanes>
 struct LogitsTile {
-    static constexpr uint32_t kStageBlocks = kN == 256 ? 1 : 2;           // K blocks of a stage
-    static constexpr uint32_t kStageBytes = kStageBlocks * (kLogitsTileTokens + kN) * 128;
-    static constexpr uint32_t kStages = kN == 128 ? 3 : 4;
+    static constexpr uint32_t kColumns = kN * kPlanes;                    // of one accumulator
+    static constexpr uint32_t kStageBlocks = kColumns < 128 ? 2 : 1;      // K blocks of a stage
+    static constexpr uint32_t kStageBytes = kStageBlocks * (kLogitsTileTokens + kColumns) * 128;
+    static constexpr uint32_t kStages = 200 * 1024 / kStageBytes;
     static constexpr uint32_t kChainStages = kChainBlocks / kStageBlocks;
     static constexpr uint32_t kPitch = kN + 4;                 // floats per row of the partial tile: no bank conflicts
     static constexpr uint32_t kDataBytes = kStages * kStageBytes;
     static_assert(kDataBytes >= kLogitsTileTokens * kPitch * 4, "the partial tile reuses the stages");
     // barriers: full[kStages], empty[kStages], acc_full[2], acc_empty[2], drain; TMEM slot, abort word
     static constexpr uint32_t kSmemBytes = 1024 + kDataBytes + (2 * kStages + 5) * 8 + 8;
-    static constexpr uint32_t kTmemColumns = 2 * kN < 32 ? 32 : 2 * kN;
+    static constexpr uint32_t kTmemStride = kColumns <= 32 ? 32 : kColumns <= 64 ? 64 : kColumns <= 128 ? 128 : 256;
+    static constexpr uint32_t kTmemColumns = 2 * kTmemStride;
 };
 
 struct LogitsMmaParams {
-    CUtensorMap x_map;            // bf16 [T][H], 128-byte swizzle: box 64 x box_tokens (x kStageBlocks)
-    CUtensorMap w_map;            // bf16 [P * E][H], box 64 x kN (x kStageBlocks)
+    CUtensorMap x_map;            // bf16 [T][H], box 64 x box_tokens, 128-byte swizzle
+    CUtensorMap w_map;            // bf16 [P * E][H], box 64 x kN
     float* out;                   // [T][E]
     uint32_t num_tokens, num_experts;
-    uint32_t k_stages, planes;    // stages that cover H; the planes alternate stage by stage
+    uint32_t k_stages;            // stages that cover H; channels past H are filled with zeros
     uint32_t box_tokens;          // rows a load of x brings: fewer than a tile when there are fewer tokens; the rest of
                                   // the tile's rows keep what shared memory held and end in rows that are not stored
-    uint32_t wide;                // 1: maps are [K/64][rows][64] views, one request per operand and stage
-    uint32_t split;               // CTAs of a cluster
+    uint32_t split;               // CTAs of a cluster: a tile's K blocks are split over them
 };
 
-// One operand of a stage: `rows` rows from `row` on, K blocks from `block` on.  Blocks past H
-// are filled with zeros.
-template <int kBlocks>
-__device__ __forceinline__ void load_operand(const CUtensorMap* map, uint32_t wide, uint32_t dst, uint32_t bar, uint32_t rows,
-                                             uint32_t row, uint32_t block, uint64_t hint) {
-    ptx::mbar_arrive_expect_tx(bar, kBlocks * rows * 128);
-    if (wide) {
-        ptx::tma_load_3d(dst, map, bar, 0, int(row), int(block), hint);
-    } else {
-#pragma unroll
-        for (uint32_t j = 0; j < kBlocks; ++j)
-            ptx::tma_load_2d(dst + j * rows * 128, map, bar, int((block + j) * kLogitsBlockK), int(row), hint);
-    }
-}
-
-template <int kN>
+template <int kN, int kPlanes>
 __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const __grid_constant__ LogitsMmaParams p) {
-    using Tile = LogitsTile<kN>;
+    using Tile = LogitsTile<kN, kPlanes>;
     constexpr uint32_t kBlocks = Tile::kStageBlocks, kStages = Tile::kStages;
     extern __shared__ uint8_t raw_smem[];
     const uint32_t base = (ptx::smem_u32(raw_smem) + 1023u) & ~1023u;     // swizzle atoms start on 1 KiB
@@ -176,10 +185,9 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = blockIdx.x;                                     // of the cluster: the K range
     const uint32_t e0 = blockIdx.y * kN, t0 = blockIdx.z * kLogitsTileTokens;
-    const uint32_t steps = p.k_stages * p.planes;
-    const uint32_t first = uint32_t(uint64_t(steps) * rank / p.split);
-    const uint32_t count = uint32_t(uint64_t(steps) * (rank + 1) / p.split) - first;   // >= 1: split <= steps
-    const uint32_t x_bytes = kBlocks * p.box_tokens * 128;                // W follows x in a stage, on a 1 KiB boundary
+    const uint32_t first = uint32_t(uint64_t(p.k_stages) * rank / p.split);
+    const uint32_t count = uint32_t(uint64_t(p.k_stages) * (rank + 1) / p.split) - first;   // >= 1: split <= k_stages
+    const uint32_t x_block = p.box_tokens * 128, x_bytes = kBlocks * x_block;   // W follows x in a stage, on a 1 KiB boundary
 
     WaitCtl ctl;
     ctl.status = g_producer_status;
@@ -203,37 +211,51 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
         *abort_word = 0;
         ptx::fence_mbar_init();
     }
-    ptx::grid_dependency_wait();
-    // TMEM only after the kernels before this one have ended: none of them can be waiting for it.
-    if (warp == 1) {
-        ptx::tmem_alloc<false>(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), Tile::kTmemColumns);
-        ptx::tmem_relinquish<false>();
-        ptx::tc_fence_before();
-    }
+    __syncwarp();
     __syncthreads();
-    ptx::tc_fence_after();
+    ptx::grid_dependency_wait();
     ptx::launch_dependents();
-    const uint32_t tmem = *tmem_slot;
+
+    uint32_t tmem = 0;
+    if (warp >= 1 && warp < 10) {
+        // The loads start meanwhile.  TMEM only after the kernels before this one have ended:
+        // none of them can be waiting for it.
+        if (warp == 1) {
+            ptx::tmem_alloc<false>(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), Tile::kTmemColumns);
+            ptx::tmem_relinquish<false>();
+            ptx::tc_fence_before();
+        }
+        asm volatile("bar.sync 1, 288;" ::: "memory");
+        ptx::tc_fence_after();
+        tmem = *tmem_slot;
+    }
 
     float acc[kN / 2];                                                    // warps 2-9: one token, half of the experts
     if (warp == 0 || warp == 10) {
         if (ptx::elect_one()) {
             // Counters instead of divisions: the loop is a chain of one thread's instructions.
-            uint32_t ks = first / p.planes, plane = first - ks * p.planes;
-            uint32_t i = 0, stage = 0, parity = 1;                        // the first round finds the stages empty
+            uint32_t i = 0, stage = 0, parity = 1, k = first * kBlocks * kLogitsBlockK;
             for (; i < count; ++i) {
                 if (i >= kStages && !mbar_wait(bar_empty + 8 * stage, parity, ctl, 1)) break;
-                const uint32_t dst = base + stage * Tile::kStageBytes, bar = bar_full + 8 * stage;
-                if (warp == 0)
-                    load_operand<kBlocks>(&p.x_map, p.wide, dst, bar, p.box_tokens, t0, ks * kBlocks, ptx::kEvictNormal);
-                else
-                    load_operand<kBlocks>(&p.w_map, p.wide, dst + x_bytes, bar, kN, plane * p.num_experts + e0, ks * kBlocks,
-                                          ptx::kEvictLast);
-                if (++plane == p.planes) { plane = 0; ++ks; }
+                const uint32_t dst = base + stage * Tile::kStageBytes;
+                const uint32_t bar = bar_full + 8 * stage;
+                ptx::mbar_arrive_expect_tx(bar, warp == 0 ? x_bytes : kBlocks * Tile::kColumns * 128);
+#pragma unroll
+                for (uint32_t j = 0; j < kBlocks; ++j) {
+                    if (warp == 0) {
+                        ptx::tma_load_2d(dst + j * x_block, &p.x_map, bar, int(k), int(t0), ptx::kEvictNormal);
+                    } else {
+#pragma unroll
+                        for (uint32_t q = 0; q < kPlanes; ++q)
+                            ptx::tma_load_2d(dst + x_bytes + (j * kPlanes + q) * kN * 128, &p.w_map, bar, int(k),
+                                             int(q * p.num_experts + e0), ptx::kEvictLast);
+                    }
+                    k += kLogitsBlockK;
+                }
                 if (++stage == kStages) { stage = 0; parity ^= 1; }
             }
             if (i < count) {
-                // Gave up: the copies in flight land (or have time to) before shared memory is used again.
+                // Gave up: the copies in flight land before shared memory is used again.
                 const uint64_t start = ptx::globaltimer_ns();
                 for (uint32_t j = i > kStages ? i - kStages : 0; j < i; ++j)
                     while (!ptx::mbar_try_wait(bar_full + 8 * (j % kStages), (j / kStages) & 1) &&
@@ -243,20 +265,19 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
         __syncwarp();
     } else if (warp == 1) {
         if (ptx::elect_one()) {
-            constexpr uint32_t idesc = ptx::instr_desc_bf16(kLogitsTileTokens, kN);
+            constexpr uint32_t idesc = ptx::instr_desc_bf16(kLogitsTileTokens, Tile::kColumns);
             const uint64_t a_desc = ptx::smem_desc(base, 1024, true), b_desc = ptx::smem_desc(base + x_bytes, 1024, true);
-            const uint32_t a_block = p.box_tokens * 128 >> 4;             // descriptors count 16-byte units
             uint32_t i = 0, stage = 0, parity = 0, chain = 0, step = 0;
             for (; i < count; ++i) {
                 const uint32_t which = chain & 1;
                 if (step == 0 && chain >= 2 && !mbar_wait(bar_acc_empty + 8 * which, ((chain >> 1) - 1) & 1, ctl, 2)) break;
                 if (!mbar_wait(bar_full + 8 * stage, parity, ctl, 3)) break;
                 ptx::tc_fence_after();
-                const uint32_t at = stage * (Tile::kStageBytes >> 4);
+                const uint32_t at = stage * (Tile::kStageBytes >> 4);     // descriptors count 16-byte units
 #pragma unroll
                 for (uint32_t j = 0; j < kBlocks; ++j)
-                    ptx::mma_bf16_k64(tmem + which * kN, a_desc + at + j * a_block, b_desc + at + j * (kN * 128 >> 4), idesc,
-                                      step + j != 0);
+                    ptx::mma_bf16_k64(tmem + which * Tile::kTmemStride, a_desc + at + j * (x_block >> 4),
+                                             b_desc + at + j * (Tile::kColumns * 128 >> 4), idesc, step + j != 0);
                 ptx::tc_commit<false>(bar_empty + 8 * stage);
                 if (++step == Tile::kChainStages || i == count - 1) {
                     ptx::tc_commit<false>(bar_acc_full + 8 * which);
@@ -274,7 +295,7 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
         }
         __syncwarp();
     } else {
-        const uint32_t half = (warp - 2) >> 2;
+        const uint32_t side = (warp - 2) >> 2;                            // half of the columns
         const uint32_t lanes = (warp & 3) << 21;                          // this warp's quarter of the TMEM lanes
         const uint32_t chains = (count + Tile::kChainStages - 1) / Tile::kChainStages;
 #pragma unroll
@@ -284,14 +305,19 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
             const bool ready = mbar_wait(bar_acc_full + 8 * (chain & 1), (chain >> 1) & 1, ctl, 4);
             if (!__all_sync(0xffffffffu, ready)) break;
             ptx::tc_fence_after();
-            const uint32_t column = tmem + lanes + (chain & 1) * kN + half * (kN / 2);
+            const uint32_t column = tmem + lanes + (chain & 1) * Tile::kTmemStride + side * (kN / 2);
 #pragma unroll
             for (int c = 0; c < kN / 2; c += 16) {
-                uint32_t r[16];
-                ptx::tmem_ld16(column + c, r);
+                uint32_t r[kPlanes][16];
+#pragma unroll
+                for (int q = 0; q < kPlanes; ++q) ptx::tmem_ld16(column + q * kN + c, r[q]);
                 ptx::tmem_ld_wait();
 #pragma unroll
-                for (int j = 0; j < 16; ++j) acc[c + j] += __uint_as_float(r[j]);
+                for (int j = 0; j < 16; ++j) {
+                    float v = __uint_as_float(r[0][j]);
+                    if constexpr (kPlanes == 3) v += __uint_as_float(r[1][j]) + __uint_as_float(r[2][j]);
+                    acc[c + j] += v;
+                }
             }
             ptx::tc_fence_before();
             __syncwarp();
@@ -303,8 +329,8 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
     // ended (the last chain's barrier), or has been drained above.
     if (warp >= 2 && warp < 10) {
         const bool failed = *abort_word != 0u;
-        const uint32_t half = (warp - 2) >> 2, token = (warp & 3) * 32 + lane;
-        float4* const row = reinterpret_cast<float4*>(smem + (token * Tile::kPitch + half * (kN / 2)) * 4);
+        const uint32_t side = (warp - 2) >> 2, token = (warp & 3) * 32 + lane;
+        float4* const row = reinterpret_cast<float4*>(smem + (token * Tile::kPitch + side * (kN / 2)) * 4);
 #pragma unroll
         for (int j = 0; j < kN / 2; j += 4)
             row[j / 4] = failed ? make_float4(NAN, NAN, NAN, NAN) : make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
@@ -317,7 +343,6 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
         if (e0 + c >= p.num_experts) continue;
         const uint32_t at = base + (r * Tile::kPitch + c) * 4;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-
         for (uint32_t s = 0; s < p.split; ++s) {
             const float4 v = ptx::ld_cluster_f32x4(ptx::mapa(at, s));
             sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
@@ -332,7 +357,7 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
                 if (e0 + c + j < p.num_experts) out[j] = v[j];
         }
     }
-    // no CTA leaves while another may still read its partial tile
+    // No CTA leaves (or frees TMEM) while another may still read its partial tile.
     __syncwarp();
     ptx::cluster_sync();
     if (warp == 1) {
