@@ -173,25 +173,28 @@ __device__ __noinline__ uint32_t group_rank_f64(const RouteParams& p, uint64_t r
     return rank;
 }
 
-// The row's choices by f64 keys (the logits themselves without a bias): lane j returns the
-// j-th expert, or -1.
+// A choice's key in 64 bits, as an integer: the logit itself without a bias.
+__device__ __forceinline__ uint64_t choice_key(const RouteParams& p, float top, double sum, float l, float b) {
+    return order_f64(p.bias != nullptr ? key_f64(p, top, sum, l, b) : double(l));
+}
+
+// The row's choices by f64 keys, one after the other, for rows with more experts in doubt
+// than a warp has lanes (most of a row alike): lane j returns the j-th expert, or -1.
 template <typename T>
-__device__ __noinline__ int choose_f64(const RouteParams& p, uint64_t row, uint32_t first, uint32_t n, bool eligible, float top) {
+__device__ __noinline__ int choose_f64(const RouteParams& p, uint64_t row, uint32_t first, uint32_t n, bool eligible, float top,
+                                       double sum) {
     constexpr uint32_t kAll = 0xffffffffu;
-    const bool keyed = p.bias != nullptr;
-    const double sum = keyed && !p.sigmoid ? row_sum_f64<T>(p, row, first, n, top) : 1.0;
-    uint64_t key[kRouteMaxPerLane];
-    for (uint32_t i = 0; i < n; ++i) {
-        float l, b;
-        const bool alive = load_logit<T>(p, row, first + i, l, b) && eligible;
-        key[i] = !alive ? 0 : order_f64(keyed ? key_f64(p, top, sum, l, b) : double(l));
-    }
+    uint64_t taken = eligible ? 0ull : ~0ull;                          // n is at most 64
     int chosen = -1;
     for (uint32_t j = 0; j < p.topk; ++j) {
         uint64_t best = 0;
         uint32_t at = 0;
-        for (uint32_t i = 0; i < n; ++i)
-            if (key[i] > best) { best = key[i]; at = i; }              // equal keys: the first
+        for (uint32_t i = 0; i < n; ++i) {
+            float l, b;
+            if ((taken >> i & 1) || !load_logit<T>(p, row, first + i, l, b)) continue;
+            const uint64_t key = choice_key(p, top, sum, l, b);
+            if (key > best) { best = key; at = i; }                    // equal keys: the first
+        }
         const uint32_t high = uint32_t(best >> 32), low = uint32_t(best);
         const uint32_t top_high = __reduce_max_sync(kAll, high);
         if (top_high == 0) break;                                      // no float orders below 2^32
@@ -199,7 +202,7 @@ __device__ __noinline__ int choose_f64(const RouteParams& p, uint64_t row, uint3
         const uint32_t winner = __ffs(__ballot_sync(kAll, high == top_high && low == top_low)) - 1;
         const uint32_t e = __shfl_sync(kAll, first + at, winner);
         if (threadIdx.x % 32 == j) chosen = int(e);
-        if (threadIdx.x % 32 == winner) key[at] = 0;
+        if (threadIdx.x % 32 == winner) taken |= 1ull << at;
     }
     return chosen;
 }
@@ -234,6 +237,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
     constexpr uint32_t kAll = 0xffffffffu;
     constexpr bool kSorted = kPerLane <= 16;
     constexpr uint32_t kPlace = kPerLane - 1u;        // bits of a key that hold the place; kPerLane is a power of two
+    __shared__ uint2 round_picks[kRouteWarps][32];
     const uint32_t lane = threadIdx.x & 31;
     const uint32_t t = blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
     ptx::launch_dependents();
@@ -344,41 +348,82 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
     for (int i = 0; i < kPerLane; ++i)
         list[i] = eligible && value[i] > -INFINITY ? (order_f32(value[i]) & ~kPlace) | (kPlace - uint32_t(i)) : 0u;
     if constexpr (kSorted) sort_descending(list);
-    uint32_t mine = 0, owner = 0, last = 0;           // lane j: the j-th choice and its lane; the best that is left
-    for (uint32_t j = 0; j <= p.topk; ++j) {
+    uint2* const picks = round_picks[threadIdx.x >> 5];
+    auto lane_best = [&]() {
         uint32_t best = list[0];
         if constexpr (!kSorted) {
 #pragma unroll
             for (int i = 1; i < kPerLane; ++i) best = max(best, list[i]);
         }
-        // without the places: of equal keys the lower lane has the lower expert
-        const uint32_t m = __reduce_max_sync(kAll, best | kPlace);
-        if (m == kPlace) break;
-        if (j == p.topk) { last = m; break; }
-        const uint32_t winner = __ffs(__ballot_sync(kAll, (best | kPlace) == m)) - 1;
-        const uint32_t key = __shfl_sync(kAll, best, winner);
-        if (lane == j) { mine = key; owner = winner; }
-        const bool won = lane == winner;
+        return best;
+    };
+    // A round: the lane with the largest key (of equal ones, the lower lane has the lower
+    // expert) writes it to a pick and passes on to its next.
+    auto round = [&](uint32_t pick, uint32_t m, uint32_t best) {
+        const bool won = lane == __ffs(__ballot_sync(kAll, (best | kPlace) == m)) - 1;
+        if (won) picks[pick] = make_uint2(best, lane);
         if constexpr (kSorted) {
 #pragma unroll
             for (int i = 0; i + 1 < kPerLane; ++i) list[i] = won ? list[i + 1] : list[i];
             list[kPerLane - 1] = won ? 0u : list[kPerLane - 1];
         } else {
 #pragma unroll
-            for (int i = 0; i < kPerLane; ++i) list[i] = won && list[i] == key ? 0u : list[i];
+            for (int i = 0; i < kPerLane; ++i) list[i] = won && list[i] == best ? 0u : list[i];
         }
+    };
+    uint32_t last = 0, count = 0;                     // the best key that is left; picks made
+    for (; count <= p.topk; ++count) {
+        const uint32_t best = lane_best(), m = __reduce_max_sync(kAll, best | kPlace);
+        last = m == kPlace ? 0u : m;                  // 0: nothing is left
+        if (last == 0 || count == p.topk) break;
+        round(count, m, best);
     }
-    const uint32_t after = __shfl_down_sync(kAll, mine, 1);
-    const uint32_t next = lane + 1 == p.topk ? last : after;
-    bool doubt = false;
-    if (lane < p.topk && mine != 0)
-        doubt = keyed ? in_doubt(mine, next, kPlace, score_error) : !kShort && (mine ^ next) <= kPlace;
-    int chosen = -1;
-    if (__any_sync(kAll, doubt)) {
-        chosen = choose_f64<T>(p, row, first, n, eligible, stats.top);
-    } else if (mine != 0) {
-        chosen = int((owner >> p.lanes_log2) * p.group_size + (owner & ((1u << p.lanes_log2) - 1u)) * p.per_lane + kPlace -
-                     (mine & kPlace));
+    __syncwarp();
+    auto order_in_doubt = [&](uint32_t a, uint32_t b) {
+        return keyed ? in_doubt(a, b, kPlace, score_error) : !kShort && (a ^ b) <= kPlace;
+    };
+    auto expert_of = [&](uint2 pick) {                // owner's group, its part of the group, place
+        return (pick.y >> p.lanes_log2) * p.group_size + (pick.y & ((1u << p.lanes_log2) - 1u)) * p.per_lane + kPlace -
+               (pick.x & kPlace);
+    };
+    uint2 pick = lane < count ? picks[lane] : make_uint2(0u, 0u);
+    const uint32_t after = __shfl_down_sync(kAll, pick.x, 1);
+    int chosen = lane < count ? int(expert_of(pick)) : -1;
+    if (__any_sync(kAll, lane < count && order_in_doubt(pick.x, lane + 1 == p.topk ? last : after))) {
+        // Exact keys for the picks and for what else may belong among them.
+        const double sum = keyed && !p.sigmoid ? row_sum_f64<T>(p, row, first, n, stats.top) : 1.0;
+        const uint32_t border = __shfl_sync(kAll, pick.x, p.topk - 1);   // the last pick, if there are that many
+        bool many = false;
+        while (count >= p.topk) {
+            const uint32_t best = lane_best(), m = __reduce_max_sync(kAll, best | kPlace);
+            if (m == kPlace || !order_in_doubt(border, m)) break;
+            many = count == 32;
+            if (many) break;
+            round(count++, m, best);
+        }
+        __syncwarp();
+        if (many) {
+            chosen = choose_f64<T>(p, row, first, n, eligible, stats.top, sum);
+        } else {
+            uint64_t key = 0;
+            uint32_t e = 0xffffffffu;
+            if (lane < count) {
+                float l, b;
+                e = expert_of(picks[lane]);
+                load_logit<T>(p, row, e, l, b);
+                key = choice_key(p, stats.top, sum, l, b);
+            }
+            uint32_t rank = 0;
+            for (uint32_t o = 0; o < count; ++o) {
+                const uint64_t k = __shfl_sync(kAll, key, o);
+                const uint32_t other = __shfl_sync(kAll, e, o);
+                rank += k > key || (k == key && other < e);
+            }
+            __syncwarp();
+            if (lane < count) picks[rank].x = e;
+            __syncwarp();
+            chosen = lane < min(count, p.topk) ? int(picks[lane].x) : -1;
+        }
     }
 
     // Weights: lane j has the j-th choice.  Renormalised scores are ratios, so they are
