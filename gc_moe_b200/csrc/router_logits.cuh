@@ -147,7 +147,7 @@ struct LogitsTile {
     static constexpr uint32_t kColumns = kN * kPlanes;                    // of one accumulator
     static constexpr uint32_t kStageBlocks = kColumns < 128 ? 2 : 1;      // K blocks of a stage
     static constexpr uint32_t kStageBytes = kStageBlocks * (kLogitsTileTokens + kColumns) * 128;
-    static constexpr uint32_t kStages = 200 * 1024 / kStageBytes;
+    static constexpr uint32_t kStages = 225 * 1024 / kStageBytes;
     static constexpr uint32_t kChainStages = kChainBlocks / kStageBlocks;
     static constexpr uint32_t kPitch = kN + 4;                 // floats per row of the partial tile: no bank conflicts
     static constexpr uint32_t kDataBytes = kStages * kStageBytes;

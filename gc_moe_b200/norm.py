@@ -16,6 +16,7 @@ import torch
 from . import _native
 from .heuristics import get_block_m_for_gc_moe
 
+_BF16 = (torch.bfloat16,)
 _FLOATS = (torch.bfloat16, torch.float32)
 
 
@@ -27,20 +28,20 @@ class NormedInputs(NamedTuple):
     residual: Optional[torch.Tensor]     # x + residual, type of the residual; None without one
 
 
-def _check_rows(t, name: str, shape, dtypes, device: int) -> None:
-    if t.dtype not in dtypes or t.shape != shape or t.get_device() != device or (shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f'{name} must be {" or ".join(str(d)[6:] for d in dtypes)} {list(shape)} on the device of x, '
-                         'contiguous in its last dimension')
+def _check_rows(t, name: str, shape, dtypes, device: int) -> int:
+    """Elements between the rows of ``t``; raise if it is not such rows."""
+    tokens, hidden = shape
+    if t.dtype not in dtypes or t.shape != shape or t.get_device() != device:
+        raise ValueError(f'{name} must be {" or ".join(str(d)[6:] for d in dtypes)} {list(shape)} on the device of x')
+    stride, one = t.stride()
+    if one != 1:
+        raise ValueError(f'{name} must be contiguous in its last dimension')
+    return stride if tokens > 1 else hidden          # a single row has no stride of its own
 
 
-def _row_stride(t: torch.Tensor, hidden: int) -> int:
-    """Elements between rows; a single row has no stride of its own."""
-    return t.stride(0) if t.shape[0] > 1 else hidden
-
-
-def _rows_like(t: torch.Tensor) -> torch.Tensor:
-    """New contiguous tensor of the shape and type of ``t``."""
-    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+def _rows_like(t: torch.Tensor, stride: int) -> torch.Tensor:
+    """New contiguous tensor of the shape and type of ``t``, whose rows are ``stride`` apart."""
+    return torch.empty_like(t) if stride == t.shape[1] else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def rms_norm_for_gc_moe(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None,
@@ -61,10 +62,11 @@ def rms_norm_for_gc_moe(x: torch.Tensor, weight: torch.Tensor, residual: Optiona
 
     Runs on the current stream and can be captured.
     """
-    if x.dim() != 2 or x.dtype != torch.bfloat16 or not x.is_cuda or x.stride(1) != 1:
+    if x.dim() != 2 or not x.is_cuda:
         raise ValueError('x must be a 2-D CUDA bfloat16 tensor, contiguous in its last dimension')
     tokens, hidden = shape = x.shape
     device = x.get_device()
+    x_stride = _check_rows(x, 'x', shape, _BF16, device)
     if hidden == 0 or hidden % 32:
         raise ValueError(f'hidden {hidden} must be a positive multiple of 32')
     if (weight.dtype not in _FLOATS or weight.shape != (hidden,) or weight.get_device() != device
@@ -72,22 +74,24 @@ def rms_norm_for_gc_moe(x: torch.Tensor, weight: torch.Tensor, residual: Optiona
         raise ValueError(f'weight must be contiguous bfloat16 or float32 [{hidden}] on the device of x')
     residual_ptr = residual_stride = residual_out_ptr = residual_out_stride = residual_f32 = 0
     if residual is not None:
-        _check_rows(residual, 'residual', shape, _FLOATS, device)
+        residual_stride = residual_out_stride = _check_rows(residual, 'residual', shape, _FLOATS, device)
         if residual_out is None:
-            residual_out = _rows_like(residual)
+            residual_out, residual_out_stride = _rows_like(residual, residual_stride), hidden
         elif residual_out is not residual:
-            _check_rows(residual_out, 'residual_out', shape, (residual.dtype,), device)
-        residual_ptr, residual_stride = residual.data_ptr(), _row_stride(residual, hidden)
-        residual_out_ptr, residual_out_stride = residual_out.data_ptr(), _row_stride(residual_out, hidden)
+            residual_out_stride = _check_rows(residual_out, 'residual_out', shape, (residual.dtype,), device)
+        residual_ptr, residual_out_ptr = residual.data_ptr(), residual_out.data_ptr()
         residual_f32 = int(residual.dtype is torch.float32)
     elif residual_out is not None:
         raise ValueError('residual_out needs a residual')
+    normed_ptr, normed_stride = 0, hidden
     if normed is True:
-        normed = _rows_like(x)
+        normed = _rows_like(x, x_stride)
+        normed_ptr = normed.data_ptr()
     elif normed is False or normed is None:
         normed = None
     else:
-        _check_rows(normed, 'normed', shape, (torch.bfloat16,), device)
+        normed_stride = _check_rows(normed, 'normed', shape, _BF16, device)
+        normed_ptr = normed.data_ptr()
     shared_sf, shared_rows, block_m = None, 0, 0
     if sym_buffer is None:
         words = (hidden + 127) // 128
@@ -109,11 +113,9 @@ def rms_norm_for_gc_moe(x: torch.Tensor, weight: torch.Tensor, residual: Optiona
             block_m = get_block_m_for_gc_moe(sym_buffer.group.size(), sym_buffer.num_experts,
                                              sym_buffer.num_max_tokens_per_rank, tokens, sym_buffer.num_topk)
     args = _native.NormArgs(
-        x.data_ptr(), residual_ptr, weight.data_ptr(), x_q.data_ptr(), x_sf.data_ptr(),
-        0 if normed is None else normed.data_ptr(), residual_out_ptr, 0 if shared_sf is None else shared_sf.data_ptr(),
-        _row_stride(x, hidden), residual_stride, 0 if normed is None else _row_stride(normed, hidden),
-        residual_out_stride, shared_rows, block_m, tokens, hidden, residual_f32,
-        int(weight.dtype is torch.float32), eps, device)
+        x.data_ptr(), residual_ptr, weight.data_ptr(), x_q.data_ptr(), x_sf.data_ptr(), normed_ptr, residual_out_ptr,
+        0 if shared_sf is None else shared_sf.data_ptr(), x_stride, residual_stride, normed_stride, residual_out_stride,
+        shared_rows, block_m, tokens, hidden, residual_f32, int(weight.dtype is torch.float32), eps, device)
     code = _native.library().gcmoe_rms_norm(ctypes.byref(args), _native.current_stream(device))
     if code:
         _native.raise_for(code)
