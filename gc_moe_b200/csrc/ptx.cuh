@@ -302,8 +302,7 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t cluster_addr) {
     float4 v;
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
                  : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                 : "r"(cluster_addr)
-                 : "memory");
+                 : "r"(cluster_addr));      // volatile: stays behind the cluster barrier
     return v;
 }
 // 32 rows x 16 bytes of shared memory -> 4 TMEM columns, replicated to the

@@ -10,9 +10,15 @@
 // The mean runs over the unrounded f32 sum h, not over the copy that is written back.
 //
 // Bound by HBM for many rows (9 + 1/32 bytes per element with a BF16 residual and both
-// outputs), by launch and load latency for few.  One CTA per row keeps the row in registers
-// between the reduction and the output, so every input is read once; a thread holds
-// kChunks x 8 consecutive channels, four lanes share one scale, sixteen one scale word.
+// outputs: 4096 x 7168 in 42.6 us, 6.2 TB/s, 95% of a copy's rate), by launch and load latency
+// for few (1 x 7168: 2.5 us, where an empty launch takes 2).  One CTA per row keeps the row in
+// registers between the reduction and the output, so every input is read once; a thread holds
+// kChunks x 8 consecutive channels, four lanes share one scale, sixteen one scale word.  With
+// up to 512 threads a row of 7168 needs 32 registers a thread, and four CTAs fit an SM: with
+// two (more registers) the same rows took 48 us.
+//
+// A group whose amax lies within f32's rounding of a border, 448 times a power of two, gets
+// one of the two scales next to it; either holds the group.
 #pragma once
 
 #include <cuda_bf16.h>

@@ -10,6 +10,7 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <type_traits>
 
 #include "device_common.cuh"
 #include "ptx.cuh"
@@ -29,7 +30,7 @@ struct LogitsParams {
 
 // Few tokens: bound by the latency of the loads, so a thread has the loads of several
 // rounds of the loop in flight.  Measured (H 7168, E 256), us for 1, 4, 8 and 16 tokens:
-// BF16 weight 2.6, 3.8, 4.1, 5.2 in this form, 5.0, 5.2, 5.2, 5.3 on the tensor cores; FP32
+// BF16 weight 2.6, 3.8, 4.1, 5.2 in this form, 4.9, 5.1, 5.1, 5.2 on the tensor cores; FP32
 // weight 4.3, 4.3, 4.5, 8.0 and 5.4, 5.7, 5.7, 5.9.
 constexpr uint32_t kFmaMaxTokens = 8;
 
@@ -125,12 +126,13 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_fma_kernel(const __grid
 // kChainBlocks K blocks (512 channels: 4.7e-7) and its accumulator is added to f32 sums in
 // registers, rounded to nearest; two accumulators in TMEM keep the MMAs going meanwhile.
 //
-// Bound by launch, TMA latency and the partial tiles' exchange for up to a few hundred tokens
-// (33 x 5120 x 384: 5.4 us), then by the traffic from L2 to the SMs: 4096 x 7168 x 256 takes
-// 20 us with 65 bytes a cycle and SM (235 MB in all; 10.2 us is what HBM needs for the inputs).
+// Bound by launch, load latency and the partial tiles' exchange for up to a few hundred
+// tokens (33 x 5120 x 384: 5.3 us, of which launch 2 and exchange and store 1), then by the
+// MMAs of 128 columns (82 cycles each, 64 at best) and the traffic from L2 to the SMs: 4096 x
+// 7168 x 256 takes 18.6 us with 235 MB brought to the SMs; the inputs need 10.2 us of HBM.
 // Tiles of 256 experts, as one CTA or as a pair with 256 tokens, move half to two thirds of
-// that but were no faster at any size: 20.8 and 22 us here, where their shared memory holds
-// too few stages to cover the latency.
+// that but were no faster at any size (20.8 and 22 us here): their shared memory holds too
+// few stages to cover the latency.
 //
 // Warp 0: loads of x; warp 1: MMAs; warps 2-9: accumulators to registers, then the sums;
 // warp 10: loads of W.
@@ -166,7 +168,7 @@ struct LogitsMmaParams {
     uint32_t k_stages;            // stages that cover H; channels past H are filled with zeros
     uint32_t box_tokens;          // rows a load of x brings: fewer than a tile when there are fewer tokens; the rest of
                                   // the tile's rows keep what shared memory held and end in rows that are not stored
-    uint32_t split;               // CTAs of a cluster: a tile's K blocks are split over them
+    uint32_t split;               // CTAs of a cluster, over which a tile's K blocks are split: 1, 2, 4 or 8
 };
 
 template <int kN, int kPlanes>
@@ -342,11 +344,21 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
         const uint32_t r = i / (kN / 4), c = i % (kN / 4) * 4;
         if (e0 + c >= p.num_experts) continue;
         const uint32_t at = base + (r * Tile::kPitch + c) * 4;
+        // in rank order; the loads of up to four ranks are in flight together
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (uint32_t s = 0; s < p.split; ++s) {
-            const float4 v = ptx::ld_cluster_f32x4(ptx::mapa(at, s));
-            sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
-        }
+        auto add_ranks = [&](uint32_t s, auto ranks) {
+            constexpr int kRanks = decltype(ranks)::value;
+            float4 v[kRanks];
+#pragma unroll
+            for (int j = 0; j < kRanks; ++j) v[j] = ptx::ld_cluster_f32x4(ptx::mapa(at, s + j));
+#pragma unroll
+            for (int j = 0; j < kRanks; ++j) { sum.x += v[j].x; sum.y += v[j].y; sum.z += v[j].z; sum.w += v[j].w; }
+        };
+        if (p.split == 1) add_ranks(0, std::integral_constant<int, 1>());
+        else if (p.split == 2) add_ranks(0, std::integral_constant<int, 2>());
+        else
+#pragma unroll 1
+            for (uint32_t s = 0; s < p.split; s += 4) add_ranks(s, std::integral_constant<int, 4>());
         float* const out = p.out + static_cast<uint64_t>(t0 + r) * p.num_experts + e0 + c;
         if (vectors) {
             *reinterpret_cast<float4*>(out) = sum;
