@@ -115,7 +115,7 @@ def rms_norm_for_gc_moe(x: torch.Tensor, weight: torch.Tensor, residual: Optiona
     args = _native.NormArgs(
         x.data_ptr(), residual_ptr, weight.data_ptr(), x_q.data_ptr(), x_sf.data_ptr(), normed_ptr, residual_out_ptr,
         0 if shared_sf is None else shared_sf.data_ptr(), x_stride, residual_stride, normed_stride, residual_out_stride,
-        shared_rows, block_m, tokens, hidden, residual_f32, int(weight.dtype is torch.float32), eps, device)
+        shared_rows, block_m, tokens, hidden, residual_f32, int(weight.dtype is torch.float32), float(eps), device)
     code = _native.library().gcmoe_rms_norm(ctypes.byref(args), _native.current_stream(device))
     if code:
         _native.raise_for(code)

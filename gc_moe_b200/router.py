@@ -59,7 +59,7 @@ def check_router_weight(router_weight, hidden, device) -> None:
 def router_logits_for_gc_moe(x: torch.Tensor, router_weight: torch.Tensor,
                              out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """FP32 ``x @ W.T`` [T, E] of BF16 ``x`` [T, H] (rows may have a stride, their
-    starts are 16-byte aligned, H is a multiple of 8) and the planes of
+    starts are 16-byte aligned, H is a multiple of 8, T at most 262140) and the planes of
     ``transform_router_weight_for_gc_moe`` [P, E, H]: exact products, FP32 sums
     in an order that depends on the sizes alone.
 
@@ -150,7 +150,7 @@ def route_for_gc_moe(logits: torch.Tensor, topk: int, *, scoring: str = 'softmax
     args = _native.RouteArgs(
         logits.data_ptr(), 0 if bias is None else bias.data_ptr(), idx.data_ptr(), weights.data_ptr(),
         logits.stride(0) if tokens > 1 else experts, tokens, experts, topk, num_groups, topk_groups,
-        _LOGIT_TYPES[logits.dtype], _SCORINGS[scoring], _GROUP_SCORES[group_score], int(bool(renormalize)), scale,
+        _LOGIT_TYPES[logits.dtype], _SCORINGS[scoring], _GROUP_SCORES[group_score], int(bool(renormalize)), float(scale),
         device, 0)
     code = _native.library().gcmoe_route(ctypes.byref(args), _native.current_stream(device))
     if code:

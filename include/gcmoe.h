@@ -226,8 +226,9 @@ typedef struct gcmoe_logits_args {
 
 /* out[t][e] = sum over planes p and channels c of x[t][c] * weight[p][e][c], f32
  * sums.  planes = 1: a bf16 router weight; planes = 3: an f32 weight split into
- * bf16 terms.  H a multiple of 8, E at most 2048.  The reference takes routing
- * decisions as inputs (README.md:234-252).  Allocates nothing; capturable. */
+ * bf16 terms.  H a multiple of 8, E at most 2048, T at most 262140.  The reference
+ * takes routing decisions as inputs (README.md:234-252).  Allocates nothing;
+ * capturable. */
 int gcmoe_router_logits(const gcmoe_logits_args* args, void* cuda_stream);
 
 /* Status words of the bounded waits inside gcmoe_router_logits, after

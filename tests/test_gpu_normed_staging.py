@@ -146,3 +146,83 @@ def test_a_wait_that_gives_up_is_reported_once(single_rank_group):
         buf.raise_on_device_error()
     finally:
         buf.destroy()
+
+
+def test_no_tokens_are_staged(single_rank_group):
+    buf = G.get_symm_buffer_for_gc_moe(single_rank_group, 8, 256, 2, 1024, 512)
+    try:
+        planes = G.transform_router_weight_for_gc_moe(torch.zeros((8, 1024), device='cuda'))
+        x = torch.empty((0, 1024), dtype=torch.bfloat16, device='cuda')
+        staged = G.stage_normed_inputs_for_gc_moe(buf, x, torch.ones(1024, device='cuda'), planes, x)
+        assert staged.normed.shape == (0, 1024) and staged.residual.shape == (0, 1024) and staged.logits.shape == (0, 8)
+    finally:
+        buf.destroy()
+
+
+def test_first_calls_of_a_process_can_be_captured():
+    """No call before the capture: nothing is set up lazily that a capture forbids."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import torch, gc_moe_b200 as G
+g = torch.Generator(device='cuda').manual_seed(1)
+x = {t: torch.randn((t, 1024), device='cuda', generator=g).to(torch.bfloat16) for t in (2, 40, 300)}
+w = torch.ones(1024, device='cuda')
+planes = G.transform_router_weight_for_gc_moe(torch.randn((64, 1024), device='cuda', generator=g) * 0.03)
+bias = torch.zeros(64, device='cuda')
+def call(t):
+    n = G.rms_norm_for_gc_moe(x[t], w, x[t])
+    logits = G.router_logits_for_gc_moe(n.normed, planes)
+    return (n.x_sf, n.normed, n.residual, logits, *G.route_for_gc_moe(logits, 4, scoring='sigmoid', bias=bias, num_groups=8, topk_groups=4))
+torch.cuda.synchronize()
+graphs = {}
+for t in x:
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        graphs[t] = (graph, call(t))
+for t, (graph, out) in graphs.items():
+    graph.replay()
+torch.cuda.synchronize()
+for t, (graph, out) in graphs.items():
+    assert all(torch.equal(a, b) for a, b in zip(out, call(t))), t
+print('captured')
+"""
+    got = subprocess.run([sys.executable, '-c', code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert got.returncode == 0 and 'captured' in got.stdout, got.stderr[-2000:]
+
+
+def test_offsets_past_32_bits():
+    """Rows 2^29 + 8 elements apart: the last ones start past 2^32 elements."""
+    rows, stride = 12, 2 ** 29 + 8
+    big = torch.zeros((rows - 1) * stride + 1024, dtype=torch.bfloat16, device='cuda')
+    x = big.as_strided((rows, 1024), (stride, 1))
+    x.copy_(torch.randn((rows, 1024)).to(torch.bfloat16))
+    near = x.contiguous()
+    w = torch.rand(1024, device='cuda')
+    planes = G.transform_router_weight_for_gc_moe(torch.randn((32, 1024), device='cuda').to(torch.bfloat16))
+    assert torch.equal(G.router_logits_for_gc_moe(x, planes), G.router_logits_for_gc_moe(near, planes))      # tensor cores
+    assert torch.equal(G.router_logits_for_gc_moe(x[5::3], planes), G.router_logits_for_gc_moe(near[5::3].contiguous(), planes))
+    for a, b in zip(G.route_for_gc_moe(x[:, :64], 8), G.route_for_gc_moe(near[:, :64], 8)):
+        assert torch.equal(a, b)
+    want = G.rms_norm_for_gc_moe(near, w, near)
+    got = G.rms_norm_for_gc_moe(x, w, x, residual_out=x)
+    assert torch.equal(got.normed, want.normed) and torch.equal(x, want.residual) and torch.equal(got.x_sf, want.x_sf)
+    del big, x, got
+    torch.cuda.empty_cache()
+
+
+def test_another_device_than_the_current_one_is_refused():
+    import ctypes
+    from gc_moe_b200 import _native
+    lib = _native.library()
+    x = torch.zeros((4, 1024), dtype=torch.bfloat16, device='cuda')
+    p, other = x.data_ptr(), torch.cuda.current_device() + 1
+    calls = ((lib.gcmoe_rms_norm, _native.NormArgs(x=p, weight=p, x_q=p, x_sf=p, x_stride=1024, num_tokens=1, hidden=1024, device=other)),
+             (lib.gcmoe_router_logits, _native.LogitsArgs(x=p, weight=p, out=p, x_stride=1024, num_tokens=1, hidden=1024, num_experts=1, planes=1, device=other)),
+             (lib.gcmoe_route, _native.RouteArgs(logits=p, topk_idx=p, topk_weights=p, logits_stride=8, num_tokens=1, num_experts=8, topk=1,
+                                                 num_groups=1, topk_groups=1, scale=1.0, device=other)))
+    for fn, args in calls:
+        assert fn(ctypes.byref(args), None) == _native.ERR_INVALID
+        assert 'current device' in _native.last_error()
