@@ -1,7 +1,9 @@
 """ctypes binding of libgcmoe_sm100.so (the C ABI declared in include/gcmoe.h).
 
 There is no fallback: if the library is missing or a call fails, the caller
-gets an exception.  The library is built by ``python -m gc_moe_b200.build``.
+gets an exception.  The library is built by ``python -m gc_moe_b200.build``, and
+so is ``_torch_binding.so``, through which the operators in front of the layer
+call it.
 """
 
 from __future__ import annotations
@@ -9,7 +11,7 @@ from __future__ import annotations
 import ctypes
 import os
 
-import torch
+import torch  # noqa: F401  (torch's libraries, which _torch_binding.so needs)
 
 MAX_RANKS = 72
 STATUS_WORDS = 8
@@ -132,10 +134,24 @@ def library() -> ctypes.CDLL:
     return _lib
 
 
-# Handle of the current stream of a device: what torch.cuda.current_stream(device).cuda_stream
-# returns, without building a Stream object (1.3 us less a call, where a launch takes 3).
-current_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (
-    lambda device: torch.cuda.current_stream(device).cuda_stream)
+_binding = None
+
+
+def binding():
+    """The compiled calls of the operators in front of the layer, bound to the
+    loaded library (``csrc/torch_binding.cpp``)."""
+    global _binding
+    if _binding is None:
+        lib = library()
+        try:
+            from . import _torch_binding
+        except ImportError as error:
+            raise RuntimeError(f'_torch_binding.so cannot be loaded ({error}): build it with '
+                               '`python -m gc_moe_b200.build`; there is no fallback path') from error
+        _torch_binding.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+            'gcmoe_rms_norm', 'gcmoe_router_logits', 'gcmoe_route', 'gcmoe_last_error')))
+        _binding = _torch_binding
+    return _binding
 
 
 def last_error() -> str:

@@ -1,9 +1,11 @@
-"""Build libgcmoe_sm100.so in-tree with nvcc for sm_100a.
+"""Build the package's native parts in-tree.
 
     python -m gc_moe_b200.build
 
-The library is the only native artefact of the package; it is loaded with
-ctypes by ``gc_moe_b200._native`` and is never rebuilt implicitly at import.
+``libgcmoe_sm100.so`` (nvcc, sm_100a) holds the kernels and the C ABI and is
+loaded with ctypes by ``gc_moe_b200._native``; ``_torch_binding.so`` (g++, torch's
+headers) takes the small calls in front of the layer from tensors to that ABI.
+Neither is ever rebuilt implicitly at import.
 """
 
 from __future__ import annotations
@@ -16,6 +18,9 @@ import sys
 PACKAGE_DIR = os.path.dirname(os.path.abspath(__file__))
 SOURCE = os.path.join(PACKAGE_DIR, 'csrc', 'gcmoe.cu')
 LIBRARY = os.path.join(PACKAGE_DIR, 'libgcmoe_sm100.so')
+BINDING_SOURCE = os.path.join(PACKAGE_DIR, 'csrc', 'torch_binding.cpp')
+BINDING = os.path.join(PACKAGE_DIR, '_torch_binding.so')
+HEADER = os.path.join(PACKAGE_DIR, '..', 'include', 'gcmoe.h')
 
 
 def _newest_source_mtime() -> float:
@@ -24,7 +29,31 @@ def _newest_source_mtime() -> float:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile the library if it is missing or older than its sources."""
+    """Compile what is missing or older than its sources; the library's path."""
+    _build_binding(force)
+    return _build_library(force, verbose)
+
+
+def _build_binding(force: bool) -> None:
+    if (not force and os.path.exists(BINDING)
+            and os.path.getmtime(BINDING) >= max(os.path.getmtime(f) for f in (BINDING_SOURCE, HEADER))):
+        return
+    import sysconfig
+    import torch
+    torch_dir = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(shutil.which('nvcc') or '/usr/local/cuda/bin/nvcc'))
+    include = [os.path.join(torch_dir, 'include'), os.path.join(torch_dir, 'include', 'torch', 'csrc', 'api', 'include'),
+               sysconfig.get_paths()['include'], os.path.join(cuda, 'include')]
+    cmd = ['g++', '-O2', '-std=c++17', '-shared', '-fPIC',
+           f'-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}', *(f'-isystem{i}' for i in include),
+           BINDING_SOURCE, '-o', BINDING, f'-L{os.path.join(torch_dir, "lib")}',
+           '-ltorch_python', '-ltorch_cpu', '-lc10', '-lc10_cuda']
+    result = subprocess.run(cmd, capture_output=True, text=True)
+    if result.returncode != 0:
+        raise RuntimeError('g++ failed:\n' + result.stdout + result.stderr)
+
+
+def _build_library(force: bool, verbose: bool) -> str:
     if (not force and os.path.exists(LIBRARY)
             and os.path.getmtime(LIBRARY) >= _newest_source_mtime()):
         return LIBRARY

@@ -759,11 +759,11 @@ static cudaError_t launch_norm(const gcmoe_norm_args& a, const NormParams& p, ui
 extern "C" int gcmoe_rms_norm(const gcmoe_norm_args* args, void* cuda_stream) {
     if (args == nullptr) return fail(GCMOE_ERR_INVALID, "null argument");
     const gcmoe_norm_args& a = *args;
-    if (a.num_tokens == 0) return GCMOE_OK;
     if (a.num_tokens > 0x7fffffffu) return fail(GCMOE_ERR_INVALID, "too many tokens");
     if (a.hidden == 0 || a.hidden % 32 || a.hidden > kNormThreads * kNormMaxChunks * 8)
         return fail(GCMOE_ERR_INVALID, "hidden must be a positive multiple of 32 up to %u", kNormThreads * kNormMaxChunks * 8);
     if (!(a.eps >= 0.f) || a.eps > 3.0e38f) return fail(GCMOE_ERR_INVALID, "eps must be a finite non-negative number");
+    if (a.num_tokens == 0) return GCMOE_OK;
     if (a.x == 0 || a.x % 16 || a.x_stride % 8 || a.weight == 0 || a.weight % 16 || a.x_q == 0 || a.x_q % 8 || a.x_sf == 0 ||
         a.x_sf % 4)
         return fail(GCMOE_ERR_INVALID, "norm input or output missing or misaligned");
@@ -900,12 +900,12 @@ static int launch_logits_mma(const gcmoe_logits_args& a, uint32_t split, cudaStr
 extern "C" int gcmoe_router_logits(const gcmoe_logits_args* args, void* cuda_stream) {
     if (args == nullptr) return fail(GCMOE_ERR_INVALID, "null argument");
     const gcmoe_logits_args& a = *args;
-    if (a.num_tokens == 0) return GCMOE_OK;
     if (a.hidden == 0 || a.hidden % 8) return fail(GCMOE_ERR_INVALID, "hidden must be a positive multiple of 8");
     if (a.num_experts == 0 || a.num_experts > uint32_t(kMaxExperts))
         return fail(GCMOE_ERR_INVALID, "num_experts must be in 1..%d", kMaxExperts);
     if (a.planes != 1 && a.planes != 3) return fail(GCMOE_ERR_INVALID, "the router weight has 1 or 3 bf16 planes");
     if (a.num_tokens > 65535u * 4u) return fail(GCMOE_ERR_INVALID, "at most %u tokens a call", 65535u * 4u);
+    if (a.num_tokens == 0) return GCMOE_OK;
     if (a.x == 0 || a.x % 16 || a.x_stride % 8 || a.weight == 0 || a.weight % 16 || a.out == 0 || a.out % 4)
         return fail(GCMOE_ERR_INVALID, "router input or output missing or misaligned");
     if (int rc = check_device(a.device)) return rc;
@@ -995,7 +995,6 @@ static auto route_kernel_for(const RouteParams& p, const gcmoe_route_args& a) ->
 extern "C" int gcmoe_route(const gcmoe_route_args* args, void* cuda_stream) {
     if (args == nullptr) return fail(GCMOE_ERR_INVALID, "null argument");
     const gcmoe_route_args& a = *args;
-    if (a.num_tokens == 0) return GCMOE_OK;
     if (a.topk == 0 || a.topk > 32) return fail(GCMOE_ERR_INVALID, "topk must be in 1..32");
     if (a.num_experts == 0 || a.num_experts > uint32_t(kMaxExperts))
         return fail(GCMOE_ERR_INVALID, "num_experts must be in 1..%d", kMaxExperts);
@@ -1007,10 +1006,6 @@ extern "C" int gcmoe_route(const gcmoe_route_args* args, void* cuda_stream) {
         return fail(GCMOE_ERR_INVALID, "topk %u exceeds the %u experts of %u groups", a.topk,
                     a.topk_groups * (a.num_experts / a.num_groups), a.topk_groups);
     if (a.logit_type > kLogitF16) return fail(GCMOE_ERR_INVALID, "logits must be f32, bf16 or f16");
-    const uint64_t width = a.logit_type == kLogitF32 ? 4 : 2;
-    if (a.logits == 0 || a.logits % width || a.bias % 4 || a.topk_idx == 0 || a.topk_idx % 8 || a.topk_weights == 0 ||
-        a.topk_weights % 4)
-        return fail(GCMOE_ERR_INVALID, "routing input or output missing or misaligned");
     if (!(a.scale >= -3.0e38f && a.scale <= 3.0e38f)) return fail(GCMOE_ERR_INVALID, "scale must be finite");
     RouteParams p = {};
     p.group_size = a.num_experts / a.num_groups;
@@ -1020,6 +1015,11 @@ extern "C" int gcmoe_route(const gcmoe_route_args* args, void* cuda_stream) {
     if (p.per_lane > kRouteMaxPerLane)
         return fail(GCMOE_ERR_UNSUPPORTED, "groups of %u experts in %u groups are too large: at most %u", p.group_size,
                     a.num_groups, kRouteMaxPerLane << p.lanes_log2);
+    if (a.num_tokens == 0) return GCMOE_OK;
+    const uint64_t width = a.logit_type == kLogitF32 ? 4 : 2;
+    if (a.logits == 0 || a.logits % width || a.bias % 4 || a.topk_idx == 0 || a.topk_idx % 8 || a.topk_weights == 0 ||
+        a.topk_weights % 4)
+        return fail(GCMOE_ERR_INVALID, "routing input or output missing or misaligned");
     if (int rc = check_device(a.device)) return rc;
     p.logits = reinterpret_cast<const void*>(a.logits);
     p.bias = reinterpret_cast<const float*>(a.bias);

@@ -8,16 +8,15 @@ and routes in its tests with a softmax over the k largest logits
 
 from __future__ import annotations
 
-import ctypes
 from typing import Optional, Tuple
 
 import torch
 
 from . import _native
 
-_LOGIT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_SCORINGS = {'softmax': 0, 'sigmoid': 1}
-_GROUP_SCORES = {'top2': 0, 'max': 1}
+_WEIGHT_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+_SCORINGS = ('softmax', 'sigmoid')
+_GROUP_SCORES = ('top2', 'max')
 
 
 def transform_router_weight_for_gc_moe(weight: torch.Tensor) -> torch.Tensor:
@@ -30,7 +29,7 @@ def transform_router_weight_for_gc_moe(weight: torch.Tensor) -> torch.Tensor:
     (a BF16 weight stored as FP32) are left out.  Call once per weight, outside
     graph capture.
     """
-    if weight.dim() != 2 or weight.dtype not in _LOGIT_TYPES:
+    if weight.dim() != 2 or weight.dtype not in _WEIGHT_TYPES:
         raise ValueError('router weight must be 2-D bfloat16, float16 or float32')
     weight = weight.detach()
     if weight.dtype == torch.bfloat16:
@@ -65,31 +64,16 @@ def router_logits_for_gc_moe(x: torch.Tensor, router_weight: torch.Tensor,
 
     Runs on the current stream and can be captured.
     """
-    if x.dim() != 2 or x.dtype != torch.bfloat16 or not x.is_cuda or x.stride(1) != 1:
-        raise ValueError('x must be a 2-D CUDA bfloat16 tensor, contiguous in its last dimension')
-    tokens, hidden = x.shape
-    device = x.get_device()
-    check_router_weight(router_weight, hidden, device)
-    planes, experts = router_weight.shape[:2]
-    if out is None:
-        out = torch.empty_strided((tokens, experts), (experts, 1), dtype=torch.float32, device=x.device)
-    elif (out.shape != (tokens, experts) or out.dtype != torch.float32 or out.get_device() != device
-          or not out.is_contiguous()):
-        raise ValueError(f'out must be contiguous float32 [{tokens}, {experts}] on the device of x')
-    args = _native.LogitsArgs(x.data_ptr(), router_weight.data_ptr(), out.data_ptr(),
-                              x.stride(0) if tokens > 1 else hidden, tokens, hidden, experts, planes, device, 0)
-    code = _native.library().gcmoe_router_logits(ctypes.byref(args), _native.current_stream(device))
-    if code:
-        _native.raise_for(code)
-    return out
+    return _native.binding().router_logits(x, router_weight, out)
 
 
 def check_routing(experts, topk, scoring, bias, num_groups, topk_groups, group_score, scale, device) -> None:
-    """Raise for options that ``gcmoe_route`` would refuse, before anything is enqueued."""
+    """Raise for options that ``route_for_gc_moe`` would refuse, for callers that
+    enqueue something before it."""
     if scoring not in _SCORINGS:
-        raise ValueError(f'scoring must be one of {tuple(_SCORINGS)}, got {scoring!r}')
+        raise ValueError(f'scoring must be one of {_SCORINGS}, got {scoring!r}')
     if group_score not in _GROUP_SCORES:
-        raise ValueError(f'group_score must be one of {tuple(_GROUP_SCORES)}, got {group_score!r}')
+        raise ValueError(f'group_score must be one of {_GROUP_SCORES}, got {group_score!r}')
     if not (0 < topk <= 32 and 0 < num_groups <= 32 and 0 < topk_groups <= num_groups and 0 < experts <= 2048
             and experts % num_groups == 0 and topk <= experts // num_groups * topk_groups):
         raise ValueError(f'invalid routing: top {topk} of {experts} experts in {topk_groups} of {num_groups} groups')
@@ -131,28 +115,10 @@ def route_for_gc_moe(logits: torch.Tensor, topk: int, *, scoring: str = 'softmax
     the workspace's ``topk_idx`` and ``topk_weights``.  Runs on the current stream
     and can be captured.
     """
-    if (logits.dim() != 2 or logits.dtype not in _LOGIT_TYPES or not logits.is_cuda
-            or (logits.shape[1] > 1 and logits.stride(1) != 1)):
-        raise ValueError('logits must be a 2-D CUDA float32, bfloat16 or float16 tensor, contiguous in its last dimension')
-    tokens, experts = logits.shape
-    device = logits.get_device()
-    if topk_groups is None:
-        topk_groups = num_groups
-    check_routing(experts, topk, scoring, bias, num_groups, topk_groups, group_score, scale, device)
-    if out is None:
-        idx = torch.empty_strided((tokens, topk), (topk, 1), dtype=torch.int64, device=logits.device)
-        weights = torch.empty_strided((tokens, topk), (topk, 1), dtype=torch.float32, device=logits.device)
-    else:
-        idx, weights = out
-        for t, dtype in ((idx, torch.int64), (weights, torch.float32)):
-            if t.shape != (tokens, topk) or t.dtype != dtype or t.get_device() != device or not t.is_contiguous():
-                raise ValueError(f'out must be contiguous int64 and float32 [{tokens}, {topk}] on the device of logits')
-    args = _native.RouteArgs(
-        logits.data_ptr(), 0 if bias is None else bias.data_ptr(), idx.data_ptr(), weights.data_ptr(),
-        logits.stride(0) if tokens > 1 else experts, tokens, experts, topk, num_groups, topk_groups,
-        _LOGIT_TYPES[logits.dtype], _SCORINGS[scoring], _GROUP_SCORES[group_score], int(bool(renormalize)), float(scale),
-        device, 0)
-    code = _native.library().gcmoe_route(ctypes.byref(args), _native.current_stream(device))
-    if code:
-        _native.raise_for(code)
-    return idx, weights
+    if scoring not in _SCORINGS or group_score not in _GROUP_SCORES:
+        raise ValueError(f'scoring must be one of {_SCORINGS} and group_score one of {_GROUP_SCORES}, got {scoring!r} and '
+                         f'{group_score!r}')
+    idx, weights = (None, None) if out is None else out
+    return _native.binding().route(logits, topk, scoring == 'sigmoid', bias, num_groups,
+                                   num_groups if topk_groups is None else topk_groups, group_score == 'max',
+                                   bool(renormalize), scale, idx, weights)

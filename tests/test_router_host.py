@@ -80,7 +80,7 @@ def test_route_argument_errors(lib):
         dict(num_experts=2040, num_groups=17, topk_groups=17)))
 
 
-def test_python_refusals_without_a_gpu():
+def test_python_refusals_without_a_gpu(lib):
     x = torch.zeros((4, 1024), dtype=torch.bfloat16)
     with pytest.raises(ValueError, match='CUDA'):
         G.rms_norm_for_gc_moe(x, torch.ones(1024))
