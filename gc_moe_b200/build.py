@@ -47,7 +47,7 @@ def _build_binding(force: bool) -> None:
     cmd = ['g++', '-O2', '-std=c++17', '-shared', '-fPIC',
            f'-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}', *(f'-isystem{i}' for i in include),
            BINDING_SOURCE, '-o', BINDING, f'-L{os.path.join(torch_dir, "lib")}',
-           '-ltorch_python', '-ltorch_cpu', '-lc10', '-lc10_cuda']
+           '-ltorch_python', '-ltorch_cuda', '-ltorch_cpu', '-lc10_cuda', '-lc10']
     result = subprocess.run(cmd, capture_output=True, text=True)
     if result.returncode != 0:
         raise RuntimeError('g++ failed:\n' + result.stdout + result.stderr)

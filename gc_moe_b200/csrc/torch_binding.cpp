@@ -9,7 +9,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/core/Tensor.h>
-#include <ATen/ops/empty_strided.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include <cmath>
@@ -56,7 +56,7 @@ bool is_rows(const at::Tensor& t, int64_t rows, int64_t columns, int device) {
 uint64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
 at::Tensor new_rows(int64_t rows, int64_t columns, at::ScalarType type, const at::Tensor& like) {
-    return at::empty_strided({rows, columns}, {columns, 1}, like.options().dtype(type));
+    return at::detail::empty_strided_cuda({rows, columns}, {columns, 1}, type, like.device());
 }
 
 void* stream_of(int device) { return c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream(); }
