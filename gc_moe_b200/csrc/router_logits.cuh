@@ -149,13 +149,19 @@ struct LogitsTile {
     static constexpr uint32_t kColumns = kN * kPlanes;                    // of one accumulator
     static constexpr uint32_t kStageBlocks = kColumns < 128 ? 2 : 1;      // K blocks of a stage
     static constexpr uint32_t kStageBytes = kStageBlocks * (kLogitsTileTokens + kColumns) * 128;
-    static constexpr uint32_t kStages = 225 * 1024 / kStageBytes;
     static constexpr uint32_t kChainStages = kChainBlocks / kStageBlocks;
-    static constexpr uint32_t kPitch = kN + 4;                 // floats per row of the partial tile: no bank conflicts
-    static constexpr uint32_t kDataBytes = kStages * kStageBytes;
-    static_assert(kDataBytes >= kLogitsTileTokens * kPitch * 4, "the partial tile reuses the stages");
+    // The partial tile that a CTA receives, row by row from every rank: its own memory where
+    // that leaves room for enough stages, else the stages' once they are done with.
+    static constexpr uint32_t kPitch = kN + 4;                 // floats per row: no bank conflicts
+    static constexpr uint32_t kPartBytes = kLogitsTileTokens * kPitch * 4;
+    static constexpr bool kApart = kN <= 64;
+    static constexpr uint32_t kStages = (224 * 1024 - (kApart ? kPartBytes : 0)) / kStageBytes;
+    static constexpr uint32_t kDataBytes = kStages * kStageBytes + (kApart ? kPartBytes : 0);
+    static constexpr uint32_t kPartOffset = kApart ? kStages * kStageBytes : 0;
+    static_assert(kPartOffset + kPartBytes <= kDataBytes, "the partial tile fits");
     // barriers: full[kStages], empty[kStages], acc_full[2], acc_empty[2], drain; TMEM slot, abort word
     static constexpr uint32_t kSmemBytes = 1024 + kDataBytes + (2 * kStages + 5) * 8 + 8;
+    static_assert(kSmemBytes <= 227 * 1024, "shared memory of an SM");
     static constexpr uint32_t kTmemStride = kColumns <= 32 ? 32 : kColumns <= 64 ? 64 : kColumns <= 128 ? 128 : 256;
     static constexpr uint32_t kTmemColumns = 2 * kTmemStride;
 };
@@ -302,11 +308,13 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
         const uint32_t chains = (count + Tile::kChainStages - 1) / Tile::kChainStages;
 #pragma unroll
         for (int j = 0; j < kN / 2; ++j) acc[j] = 0.f;
+        bool arrived = false;
         for (uint32_t chain = 0; chain < chains; ++chain) {
             // all lanes wait alike; a warp leaves as a whole
             const bool ready = mbar_wait(bar_acc_full + 8 * (chain & 1), (chain >> 1) & 1, ctl, 4);
             if (!__all_sync(0xffffffffu, ready)) break;
             ptx::tc_fence_after();
+            if (!Tile::kApart && chain == chains - 1) { ptx::cluster_arrive(); arrived = true; }
             const uint32_t column = tmem + lanes + (chain & 1) * Tile::kTmemStride + side * (kN / 2);
 #pragma unroll
             for (int c = 0; c < kN / 2; c += 16) {
@@ -325,40 +333,45 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(bar_acc_empty + 8 * (chain & 1));
         }
+        if (!Tile::kApart && !arrived) ptx::cluster_arrive();
     }
+    if (!Tile::kApart && (warp < 2 || warp == 10)) ptx::cluster_arrive();
+    ptx::tc_fence_before();
     __syncthreads();
-    // The partial tile replaces the stages: every load has been consumed and every MMA has
-    // ended (the last chain's barrier), or has been drained above.
+    // Every load has been consumed and every MMA has ended (the last chain's barrier), or has
+    // been drained above.  Row r of the tile belongs to rank r % split, at place r / split of
+    // its part for each sender.  Where the parts lie in the stages, every CTA of the cluster
+    // has told that it is done with them: its loading and MMA warps at their end, the others
+    // when the last chain was complete.
+    if constexpr (!Tile::kApart) ptx::cluster_wait();
+    const uint32_t part = base + Tile::kPartOffset, owned = kLogitsTileTokens / p.split;
     if (warp >= 2 && warp < 10) {
         const bool failed = *abort_word != 0u;
         const uint32_t side = (warp - 2) >> 2, token = (warp & 3) * 32 + lane;
-        float4* const row = reinterpret_cast<float4*>(smem + (token * Tile::kPitch + side * (kN / 2)) * 4);
+        const uint32_t at = part + ((rank * owned + token / p.split) * Tile::kPitch + side * (kN / 2)) * 4;
+        const uint32_t to = ptx::mapa(at, token % p.split);
 #pragma unroll
         for (int j = 0; j < kN / 2; j += 4)
-            row[j / 4] = failed ? make_float4(NAN, NAN, NAN, NAN) : make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+            ptx::st_cluster_f32x4(to + j * 4, failed ? make_float4(NAN, NAN, NAN, NAN)
+                                                     : make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]));
+    } else if (warp == 1) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc<false>(tmem, Tile::kTmemColumns);
     }
+    __syncwarp();
+    // After this no CTA touches another's memory.
     ptx::cluster_sync();
     const uint32_t rows = min(kLogitsTileTokens, p.num_tokens - t0);
     const bool vectors = p.num_experts % 4 == 0;
-    for (uint32_t i = rank * kLogitsMmaThreads + tid; i < rows * (kN / 4); i += p.split * kLogitsMmaThreads) {
-        const uint32_t r = i / (kN / 4), c = i % (kN / 4) * 4;
-        if (e0 + c >= p.num_experts) continue;
-        const uint32_t at = base + (r * Tile::kPitch + c) * 4;
-        // in rank order; the loads of up to four ranks are in flight together
+    for (uint32_t i = tid; i < owned * (kN / 4); i += kLogitsMmaThreads) {
+        const uint32_t place = i / (kN / 4), r = place * p.split + rank, c = i % (kN / 4) * 4;
+        if (r >= rows || e0 + c >= p.num_experts) continue;
+        const float* const from = reinterpret_cast<const float*>(smem + Tile::kPartOffset) + place * Tile::kPitch + c;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        auto add_ranks = [&](uint32_t s, auto ranks) {
-            constexpr int kRanks = decltype(ranks)::value;
-            float4 v[kRanks];
-#pragma unroll
-            for (int j = 0; j < kRanks; ++j) v[j] = ptx::ld_cluster_f32x4(ptx::mapa(at, s + j));
-#pragma unroll
-            for (int j = 0; j < kRanks; ++j) { sum.x += v[j].x; sum.y += v[j].y; sum.z += v[j].z; sum.w += v[j].w; }
-        };
-        if (p.split == 1) add_ranks(0, std::integral_constant<int, 1>());
-        else if (p.split == 2) add_ranks(0, std::integral_constant<int, 2>());
-        else
-#pragma unroll 1
-            for (uint32_t s = 0; s < p.split; s += 4) add_ranks(s, std::integral_constant<int, 4>());
+        for (uint32_t s = 0; s < p.split; ++s) {                          // in rank order
+            const float4 v = *reinterpret_cast<const float4*>(from + s * owned * Tile::kPitch);
+            sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+        }
         float* const out = p.out + static_cast<uint64_t>(t0 + r) * p.num_experts + e0 + c;
         if (vectors) {
             *reinterpret_cast<float4*>(out) = sum;
@@ -368,13 +381,6 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
             for (uint32_t j = 0; j < 4; ++j)
                 if (e0 + c + j < p.num_experts) out[j] = v[j];
         }
-    }
-    // No CTA leaves (or frees TMEM) while another may still read its partial tile.
-    __syncwarp();
-    ptx::cluster_sync();
-    if (warp == 1) {
-        ptx::tc_fence_after();
-        ptx::tmem_dealloc<false>(tmem, Tile::kTmemColumns);
     }
 }
 
