@@ -837,15 +837,17 @@ static cudaError_t launch_logits_fma(const LogitsParams& p, cudaStream_t s) {
 struct LogitsPlan {
     uint32_t experts, split;
 };
+static uint32_t logits_tile_tokens(uint32_t tokens) { return tokens <= 64 ? 64 : kLogitsMaxTokens; }
 static LogitsPlan plan_logits(uint32_t tokens, uint32_t experts, uint32_t hidden, uint32_t planes) {
     const uint64_t blocks = (hidden + kLogitsBlockK - 1) / kLogitsBlockK;
-    const uint32_t rows = tokens < kLogitsTileTokens ? tokens : kLogitsTileTokens;
+    const uint32_t tile = logits_tile_tokens(tokens), rows = tokens < tile ? tokens : tile;
     LogitsPlan best = {32, 1};
     uint64_t least = ~0ull;
+    const uint32_t most = (planes == 1 ? 128u : 64u) / (tile == 64 ? 2u : 1u);
     for (uint32_t split = 1; split <= 8 && (split == 1 || split <= blocks / 2); split *= 2) {
-        for (uint32_t n = 32; n <= (planes == 1 ? 128u : 64u) && (n == 32 || n / 2 < experts); n *= 2) {
+        for (uint32_t n = 32; n <= most && (n == 32 || n / 2 < experts); n *= 2) {
             const uint32_t columns = n * planes;
-            const uint64_t ctas = uint64_t((tokens + kLogitsTileTokens - 1) / kLogitsTileTokens) * ((experts + n - 1) / n) * split;
+            const uint64_t ctas = uint64_t((tokens + tile - 1) / tile) * ((experts + n - 1) / n) * split;
             const uint64_t room = split == 8 ? 112 : split == 4 ? 132 : 148;
             const uint64_t waves = (ctas + room - 1) / room, steps = (blocks + split - 1) / split;
             const uint64_t bytes = (rows + columns) * 128 / 65;
@@ -857,11 +859,11 @@ static LogitsPlan plan_logits(uint32_t tokens, uint32_t experts, uint32_t hidden
     return best;
 }
 
-template <int kN, int kPlanes>
+template <int kM, int kN, int kPlanes>
 static int launch_logits_mma(const gcmoe_logits_args& a, uint32_t split, cudaStream_t s) {
-    using Tile = LogitsTile<kN, kPlanes>;
+    using Tile = LogitsTile<kM, kN, kPlanes>;
     LogitsMmaParams p;
-    p.box_tokens = a.num_tokens < kLogitsTileTokens ? round_up_u32(a.num_tokens, 8) : kLogitsTileTokens;
+    p.box_tokens = a.num_tokens < kM ? round_up_u32(a.num_tokens, 8) : kM;
     const uint64_t x_dims[2] = {a.hidden, a.num_tokens}, w_dims[2] = {a.hidden, uint64_t(kPlanes) * a.num_experts};
     const uint64_t x_pitch = a.x_stride * 2, w_pitch = uint64_t(a.hidden) * 2;
     const uint32_t x_box[2] = {kLogitsBlockK, p.box_tokens}, w_box[2] = {kLogitsBlockK, kN};
@@ -876,12 +878,12 @@ static int launch_logits_mma(const gcmoe_logits_args& a, uint32_t split, cudaStr
     static std::atomic<uint64_t> ready{0};
     const uint64_t bit = 1ull << (a.device & 63);
     if (!(ready.load() & bit)) {
-        GCMOE_CUDA(cudaFuncSetAttribute(logits_mma_kernel<kN, kPlanes>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        GCMOE_CUDA(cudaFuncSetAttribute(logits_mma_kernel<kM, kN, kPlanes>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                         Tile::kSmemBytes));
         ready |= bit;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(split, (a.num_experts + kN - 1) / kN, (a.num_tokens + kLogitsTileTokens - 1) / kLogitsTileTokens);
+    cfg.gridDim = dim3(split, (a.num_experts + kN - 1) / kN, (a.num_tokens + kM - 1) / kM);
     cfg.blockDim = dim3(kLogitsMmaThreads);
     cfg.dynamicSmemBytes = Tile::kSmemBytes;
     cfg.stream = s;
@@ -893,7 +895,7 @@ static int launch_logits_mma(const gcmoe_logits_args& a, uint32_t split, cudaStr
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    GCMOE_CUDA(cudaLaunchKernelEx(&cfg, logits_mma_kernel<kN, kPlanes>, p));
+    GCMOE_CUDA(cudaLaunchKernelEx(&cfg, logits_mma_kernel<kM, kN, kPlanes>, p));
     return GCMOE_OK;
 }
 
@@ -928,13 +930,17 @@ extern "C" int gcmoe_router_logits(const gcmoe_logits_args* args, void* cuda_str
         return GCMOE_OK;
     }
     const LogitsPlan plan = plan_logits(a.num_tokens, a.num_experts, a.hidden, a.planes);
+    if (logits_tile_tokens(a.num_tokens) == 64) {
+        if (a.planes == 3) return launch_logits_mma<64, 32, 3>(a, plan.split, s);
+        return plan.experts == 32 ? launch_logits_mma<64, 32, 1>(a, plan.split, s) : launch_logits_mma<64, 64, 1>(a, plan.split, s);
+    }
     if (a.planes == 3)
-        return plan.experts == 32 ? launch_logits_mma<32, 3>(a, plan.split, s)
-                                  : launch_logits_mma<64, 3>(a, plan.split, s);
+        return plan.experts == 32 ? launch_logits_mma<128, 32, 3>(a, plan.split, s)
+                                  : launch_logits_mma<128, 64, 3>(a, plan.split, s);
     switch (plan.experts) {
-        case 32: return launch_logits_mma<32, 1>(a, plan.split, s);
-        case 64: return launch_logits_mma<64, 1>(a, plan.split, s);
-        default: return launch_logits_mma<128, 1>(a, plan.split, s);
+        case 32: return launch_logits_mma<128, 32, 1>(a, plan.split, s);
+        case 64: return launch_logits_mma<128, 64, 1>(a, plan.split, s);
+        default: return launch_logits_mma<128, 128, 1>(a, plan.split, s);
     }
 }
 

@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_fma_kernel(const __grid
 }
 
 // ---------------------------------------------------------------------------------------
-// Tensor-core form, for more than a few tokens: tiles of 128 tokens x kN experts, the K
+// Tensor-core form, for more than a few tokens: tiles of kM tokens x kN experts, the K
 // blocks (64 channels) of a tile split over CTAs of a cluster, whose partial tiles are added
 // through distributed shared memory in rank order.
 //
@@ -137,23 +137,23 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_fma_kernel(const __grid
 // Warp 0: loads of x; warp 1: MMAs; warps 2-9: accumulators to registers, then the sums;
 // warp 10: loads of W.
 constexpr uint32_t kLogitsMmaThreads = 352;
-constexpr uint32_t kLogitsTileTokens = 128;
+constexpr uint32_t kLogitsMaxTokens = 128;           // of a tile
 constexpr uint32_t kLogitsBlockK = 64;
 constexpr uint32_t kChainBlocks = 8;
 
 // Where a wait of these launches gave up, for gcmoe_producer_status (they have no plan).
 static __device__ uint32_t g_producer_status[kStatusWords];
 
-template <int kN, int kPlanes>
+template <int kM, int kN, int kPlanes>
 struct LogitsTile {
     static constexpr uint32_t kColumns = kN * kPlanes;                    // of one accumulator
     static constexpr uint32_t kStageBlocks = kColumns < 128 ? 2 : 1;      // K blocks of a stage
-    static constexpr uint32_t kStageBytes = kStageBlocks * (kLogitsTileTokens + kColumns) * 128;
+    static constexpr uint32_t kStageBytes = kStageBlocks * (kM + kColumns) * 128;
     static constexpr uint32_t kChainStages = kChainBlocks / kStageBlocks;
     // The partial tile that a CTA receives, row by row from every rank: its own memory where
     // that leaves room for enough stages, else the stages' once they are done with.
     static constexpr uint32_t kPitch = kN + 4;                 // floats per row: no bank conflicts
-    static constexpr uint32_t kPartBytes = kLogitsTileTokens * kPitch * 4;
+    static constexpr uint32_t kPartBytes = kM * kPitch * 4;
     static constexpr bool kApart = kN <= 64;
     static constexpr uint32_t kStages = (224 * 1024 - (kApart ? kPartBytes : 0)) / kStageBytes;
     static constexpr uint32_t kDataBytes = kStages * kStageBytes + (kApart ? kPartBytes : 0);
@@ -177,9 +177,9 @@ struct LogitsMmaParams {
     uint32_t split;               // CTAs of a cluster, over which a tile's K blocks are split: 1, 2, 4 or 8
 };
 
-template <int kN, int kPlanes>
+template <int kM, int kN, int kPlanes>
 __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const __grid_constant__ LogitsMmaParams p) {
-    using Tile = LogitsTile<kN, kPlanes>;
+    using Tile = LogitsTile<kM, kN, kPlanes>;
     constexpr uint32_t kBlocks = Tile::kStageBlocks, kStages = Tile::kStages;
     extern __shared__ uint8_t raw_smem[];
     const uint32_t base = (ptx::smem_u32(raw_smem) + 1023u) & ~1023u;     // swizzle atoms start on 1 KiB
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
 
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = blockIdx.x;                                     // of the cluster: the K range
-    const uint32_t e0 = blockIdx.y * kN, t0 = blockIdx.z * kLogitsTileTokens;
+    const uint32_t e0 = blockIdx.y * kN, t0 = blockIdx.z * kM;
     const uint32_t first = uint32_t(uint64_t(p.k_stages) * rank / p.split);
     const uint32_t count = uint32_t(uint64_t(p.k_stages) * (rank + 1) / p.split) - first;   // >= 1: split <= k_stages
     const uint32_t x_block = p.box_tokens * 128, x_bytes = kBlocks * x_block;   // W follows x in a stage, on a 1 KiB boundary
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
         __syncwarp();
     } else if (warp == 1) {
         if (ptx::elect_one()) {
-            constexpr uint32_t idesc = ptx::instr_desc_bf16(kLogitsTileTokens, Tile::kColumns);
+            constexpr uint32_t idesc = ptx::instr_desc_bf16(kM, Tile::kColumns);
             const uint64_t a_desc = ptx::smem_desc(base, 1024, true), b_desc = ptx::smem_desc(base + x_bytes, 1024, true);
             uint32_t i = 0, stage = 0, parity = 0, chain = 0, step = 0;
             for (; i < count; ++i) {
@@ -344,12 +344,14 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
     // has told that it is done with them: its loading and MMA warps at their end, the others
     // when the last chain was complete.
     if constexpr (!Tile::kApart) ptx::cluster_wait();
-    const uint32_t part = base + Tile::kPartOffset, owned = kLogitsTileTokens / p.split;
+    const uint32_t part = base + Tile::kPartOffset, owned = kM / p.split;
     if (warp >= 2 && warp < 10) {
         const bool failed = *abort_word != 0u;
-        const uint32_t side = (warp - 2) >> 2, token = (warp & 3) * 32 + lane;
+        // an accumulator of 64 rows has 16 of them in the first half of each quarter of the lanes
+        const uint32_t side = (warp - 2) >> 2, token = kM == 128 ? (warp & 3) * 32 + lane : (warp & 3) * 16 + (lane & 15);
         const uint32_t at = part + ((rank * owned + token / p.split) * Tile::kPitch + side * (kN / 2)) * 4;
         const uint32_t to = ptx::mapa(at, token % p.split);
+        if (kM == 128 || lane < 16)
 #pragma unroll
         for (int j = 0; j < kN / 2; j += 4)
             ptx::st_cluster_f32x4(to + j * 4, failed ? make_float4(NAN, NAN, NAN, NAN)
@@ -361,7 +363,7 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
     __syncwarp();
     // After this no CTA touches another's memory.
     ptx::cluster_sync();
-    const uint32_t rows = min(kLogitsTileTokens, p.num_tokens - t0);
+    const uint32_t rows = min(kM, p.num_tokens - t0);
     const bool vectors = p.num_experts % 4 == 0;
     for (uint32_t i = tid; i < owned * (kN / 4); i += kLogitsMmaThreads) {
         const uint32_t place = i / (kN / 4), r = place * p.split + rank, c = i % (kN / 4) * 4;
