@@ -827,33 +827,37 @@ static cudaError_t launch_logits_fma(const LogitsParams& p, cudaStream_t s) {
 }
 
 // Tile and split of the tensor-core form: the choice with the least estimated time, in
-// cycles.  A K block costs the bytes it brings from L2 (65 a cycle and SM with all SMs at it)
-// or its four MMAs, whichever is longer; a launch its waves over the SMs (clusters leave some
-// SMs of a GPC unused), a fixed start and end, and the partial tiles' way through shared
-// memory.  Over 24 sizes (1 to 4096 tokens, 64 to 384 experts, H 1056 to 7168, both weight
-// types) the choice was within 5% of the best of all tiles and splits, measured one by one:
-// 128 x 7168 x 256, for one, 6.2 us with 32 experts over 8 CTAs, 9.8 with 128 over 4;
-// 2048 x 7168 x 256 the other way round, 13.2 us with 128 over 4, 20 with 64 over 4.
+// cycles.  A K block costs the bytes it brings from L2 (9500 a cycle shared by the CTAs, at
+// most 95 each) or its four MMAs (measured per tile), whichever is longer; a launch its waves
+// over the SMs (clusters leave some SMs of a GPC unused), a fixed start and end, and the
+// partial tiles' way to their owners and out.  Over 27 sizes (9 to 4096 tokens, 64 to 384
+// experts, H 1056 to 7168, both weight types) the choice was within 5% of the best of all
+// tiles and splits, measured one by one, and 0.2% off on average: 128 x 7168 x 256, for one,
+// takes 5.1 us with 64 x 64 over 8 CTAs and 6.7 with 128 x 32 over 4; 2048 x 7168 x 256 takes
+// 13.4 with 128 x 128 over 4 and 16.8 with 64 x 64 over 1.
 struct LogitsPlan {
-    uint32_t experts, split;
+    uint32_t tokens, experts, split;
 };
-static uint32_t logits_tile_tokens(uint32_t tokens) { return tokens <= 64 ? 64 : kLogitsMaxTokens; }
 static LogitsPlan plan_logits(uint32_t tokens, uint32_t experts, uint32_t hidden, uint32_t planes) {
-    const uint64_t blocks = (hidden + kLogitsBlockK - 1) / kLogitsBlockK;
-    const uint32_t tile = logits_tile_tokens(tokens), rows = tokens < tile ? tokens : tile;
-    LogitsPlan best = {32, 1};
-    uint64_t least = ~0ull;
-    const uint32_t most = (planes == 1 ? 128u : 64u) / (tile == 64 ? 2u : 1u);
-    for (uint32_t split = 1; split <= 8 && (split == 1 || split <= blocks / 2); split *= 2) {
+    const uint32_t blocks = (hidden + kLogitsBlockK - 1) / kLogitsBlockK;
+    LogitsPlan best = {64, 32, 1};
+    double least = 1e300;
+    for (uint32_t m = 64; m <= 128 && (m == 64 || tokens > 64); m *= 2) {
+        const uint32_t rows = tokens < m ? tokens : m, most = planes == 1 && m == 128 ? 128 : 64;
         for (uint32_t n = 32; n <= most && (n == 32 || n / 2 < experts); n *= 2) {
             const uint32_t columns = n * planes;
-            const uint64_t ctas = uint64_t((tokens + tile - 1) / tile) * ((experts + n - 1) / n) * split;
-            const uint64_t room = split == 8 ? 112 : split == 4 ? 132 : 148;
-            const uint64_t waves = (ctas + room - 1) / room, steps = (blocks + split - 1) / split;
-            const uint64_t bytes = (rows + columns) * 128 / 65;
-            const uint64_t mma = columns <= 96 ? 230 : columns == 128 ? 320 : 410;
-            const uint64_t time = waves * (steps * (bytes > mma ? bytes : mma) + 6500 + rows * n / 4);
-            if (time < least) { least = time; best = {n, split}; }
+            const double mma = m == 64 ? (columns <= 64 ? 190 : columns == 96 ? 215 : 380)
+                                       : (columns <= 96 ? 225 : columns == 128 ? 320 : 410);
+            for (uint32_t split = 1; split <= 8 && (split == 1 || split <= blocks / 2); split *= 2) {
+                const uint64_t ctas = uint64_t((tokens + m - 1) / m) * ((experts + n - 1) / n) * split;
+                const uint64_t room = split == 8 ? 112 : split == 4 ? 132 : 148;
+                const double waves = double((ctas + room - 1) / room), steps = (blocks + split - 1) / split;
+                const double share = 9500.0 / double(ctas < 148 ? ctas : 148), rate = share < 95 ? share : 95;
+                const double loads = (rows + columns) * 128 / rate;
+                const double time = waves * (steps * (loads > mma ? loads : mma) + 4500 +
+                                             rows * n * (0.2 + 0.1 * (split - 1) / split));
+                if (time < least) { least = time; best = {m, n, split}; }
+            }
         }
     }
     return best;
@@ -930,8 +934,9 @@ extern "C" int gcmoe_router_logits(const gcmoe_logits_args* args, void* cuda_str
         return GCMOE_OK;
     }
     const LogitsPlan plan = plan_logits(a.num_tokens, a.num_experts, a.hidden, a.planes);
-    if (logits_tile_tokens(a.num_tokens) == 64) {
-        if (a.planes == 3) return launch_logits_mma<64, 32, 3>(a, plan.split, s);
+    if (plan.tokens == 64) {
+        if (a.planes == 3)
+            return plan.experts == 32 ? launch_logits_mma<64, 32, 3>(a, plan.split, s) : launch_logits_mma<64, 64, 3>(a, plan.split, s);
         return plan.experts == 32 ? launch_logits_mma<64, 32, 1>(a, plan.split, s) : launch_logits_mma<64, 64, 1>(a, plan.split, s);
     }
     if (a.planes == 3)

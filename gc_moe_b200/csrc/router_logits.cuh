@@ -30,8 +30,8 @@ struct LogitsParams {
 
 // Few tokens: bound by the latency of the loads, so a thread has the loads of several
 // rounds of the loop in flight.  Measured (H 7168, E 256), us for 1, 4, 8 and 16 tokens:
-// BF16 weight 2.6, 3.8, 4.1, 5.2 in this form, 4.9, 5.1, 5.1, 5.2 on the tensor cores; FP32
-// weight 4.3, 4.3, 4.5, 8.0 and 5.4, 5.7, 5.7, 5.9.
+// BF16 weight 2.6, 3.8, 4.1, 5.2 in this form, 4.3, 4.3, 4.3, 4.3 on the tensor cores; FP32
+// weight 4.3, 4.3, 4.5, 8.0 and 4.8, 4.8, 4.8, 4.9.
 constexpr uint32_t kFmaMaxTokens = 8;
 
 template <int kTokens, int kPlanes>
@@ -127,12 +127,13 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_fma_kernel(const __grid
 // registers, rounded to nearest; two accumulators in TMEM keep the MMAs going meanwhile.
 //
 // Bound by launch, load latency and the partial tiles' exchange for up to a few hundred
-// tokens (33 x 5120 x 384: 5.3 us, of which launch 2 and exchange and store 1), then by the
-// MMAs of 128 columns (82 cycles each, 64 at best) and the traffic from L2 to the SMs: 4096 x
-// 7168 x 256 takes 18.6 us with 235 MB brought to the SMs; the inputs need 10.2 us of HBM.
-// Tiles of 256 experts, as one CTA or as a pair with 256 tokens, move half to two thirds of
-// that but were no faster at any size (20.8 and 22 us here): their shared memory holds too
-// few stages to cover the latency.
+// tokens (33 x 5120 x 384: 4.1 us, of which an empty launch takes 2), then by the MMAs (82
+// cycles for 128 x 128, 64 at best) and the traffic from L2 to the SMs: 4096 x 7168 x 256 takes
+// 18.8 us with 235 MB brought to the SMs; the inputs need 10.2 us of HBM.  Tiles of 256
+// experts, as one CTA or as a pair with 256 tokens, move half to two thirds of that but were
+// no faster at any size (20.8 and 22 us here): their shared memory holds too few stages to
+// cover the latency.  An MMA of 64 rows takes half the time of one of 128, and its smaller
+// stages hold most of a CTA's K range at once.
 //
 // Warp 0: loads of x; warp 1: MMAs; warps 2-9: accumulators to registers, then the sums;
 // warp 10: loads of W.

@@ -41,7 +41,8 @@ def _check_logits(got, x, w):
 @pytest.mark.parametrize('tokens,hidden,experts', [
     (1, 8, 1), (1, 7168, 256), (2, 1024, 8), (3, 1032, 7), (4, 5120, 384), (7, 2056, 33), (8, 4096, 64), (13, 6144, 255),
     (16, 7168, 256), (17, 7168, 256), (31, 4104, 65), (64, 512, 130), (129, 7168, 256), (200, 64, 300), (257, 1064, 257),
-    (1000, 5120, 384), (40, 2048, 2048), (2100, 2048, 256), (700, 1096, 250), (4097, 136, 40), (130, 7168, 512)])
+    (1000, 5120, 384), (40, 2048, 2048), (2100, 2048, 256), (700, 1096, 250), (4097, 136, 40), (130, 7168, 512),
+    (300, 7168, 384), (96, 7168, 256), (63, 72, 500), (65, 1000, 129)])
 def test_logits_against_the_formula(tokens, hidden, experts, weight):
     x, w = _logits_case(tokens, hidden, experts, weight, seed=tokens + experts)
     planes = G.transform_router_weight_for_gc_moe(w.cuda())
