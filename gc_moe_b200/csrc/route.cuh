@@ -354,6 +354,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
         list[i] = eligible && value[i] > -INFINITY ? (order_f32(value[i]) & ~kPlace) | (kPlace - uint32_t(i)) : 0u;
     if constexpr (kSorted) sort_descending(list);
     uint2* const picks = round_picks[threadIdx.x >> 5];
+    const uint32_t lower_lanes = (1u << lane) - 1u;
     auto lane_best = [&]() {
         uint32_t best = list[0];
         if constexpr (!kSorted) {
@@ -365,7 +366,9 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
     // A round: the lane with the largest key (of equal ones, the lower lane has the lower
     // expert) writes it to a pick and passes on to its next.
     auto round = [&](uint32_t pick, uint32_t m, uint32_t best) {
-        const bool won = lane == __ffs(__ballot_sync(kAll, (best | kPlace) == m)) - 1;
+        const bool alike = (best | kPlace) == m;
+        const uint32_t all_alike = __ballot_sync(kAll, alike);         // by every lane: not inside a condition
+        const bool won = alike && (all_alike & lower_lanes) == 0;
         if (won) picks[pick] = make_uint2(best, lane);
         if constexpr (kSorted) {
 #pragma unroll
@@ -376,13 +379,13 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
             for (int i = 0; i < kPerLane; ++i) list[i] = won && list[i] == best ? 0u : list[i];
         }
     };
-    uint32_t last = 0, count = 0;                     // the best key that is left; picks made
-    for (; count <= p.topk; ++count) {
-        const uint32_t best = lane_best(), m = __reduce_max_sync(kAll, best | kPlace);
-        last = m == kPlace ? 0u : m;                  // 0: nothing is left
-        if (last == 0 || count == p.topk) break;
-        round(count, m, best);
+    uint32_t count = 0;                               // picks made
+    uint32_t m = __reduce_max_sync(kAll, lane_best() | kPlace);
+    while (count < p.topk && m != kPlace) {           // kPlace: nothing is left
+        round(count++, m, lane_best());
+        m = __reduce_max_sync(kAll, lane_best() | kPlace);
     }
+    const uint32_t last = m == kPlace ? 0u : m;       // the best key that is left
     __syncwarp();
     auto order_in_doubt = [&](uint32_t a, uint32_t b) {
         return keyed ? in_doubt(a, b, kPlace, score_error) : !kShort && (a ^ b) <= kPlace;
@@ -399,12 +402,11 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
         const double sum = keyed && !p.sigmoid ? row_sum_f64<T>(p, row, first, n, stats.top) : 1.0;
         const uint32_t border = __shfl_sync(kAll, pick.x, p.topk - 1);   // the last pick, if there are that many
         bool many = false;
-        while (count >= p.topk) {
-            const uint32_t best = lane_best(), m = __reduce_max_sync(kAll, best | kPlace);
-            if (m == kPlace || !order_in_doubt(border, m)) break;
+        while (count >= p.topk && m != kPlace && order_in_doubt(border, m)) {
             many = count == 32;
             if (many) break;
-            round(count++, m, best);
+            round(count++, m, lane_best());
+            m = __reduce_max_sync(kAll, lane_best() | kPlace);
         }
         __syncwarp();
         if (many) {
@@ -439,14 +441,18 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
     float weight = 0.f;
     if (p.renormalize) {
         const float peak = unorder_f32(__reduce_max_sync(kAll, order_f32(l)));
-        if (chosen >= 0) {
-            weight = p.sigmoid && l > 0.f ? 1.f : expf(l - (p.sigmoid ? fminf(peak, 0.f) : peak));
-            if (p.sigmoid) weight /= 1.f + expf(-fabsf(l));
+        if (p.sigmoid) {
+            const float z = expf(-fabsf(l));          // -inf (no choice): 0
+            weight = l > 0.f ? 1.f : peak > 0.f ? z : expf(l - peak);
+            weight = __fdividef(weight, 1.f + z);
+        } else {
+            weight = expf(l - peak);
         }
+        if (chosen < 0) weight = 0.f;
         float sum = weight;
 #pragma unroll
         for (uint32_t d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(kAll, sum, d);
-        if (chosen >= 0) weight /= sum;
+        if (chosen >= 0) weight = __fdividef(weight, sum);
     } else if (chosen >= 0) {
         weight = p.sigmoid ? sigmoid_f32(l) : expf(l - stats.top) / stats.sum;
     }
