@@ -20,16 +20,16 @@
 // are integers that order like the floats (0 = not eligible) whose lowest bits are replaced
 // by the expert's place in its lane, so that equal keys go to the lower expert and a
 // minimum or maximum moves key and expert together: a lane's list is sorted with two
-// instructions per comparison, and a round of the selection is one redux.max, a ballot and a
-// shift of the winner's list.  The replaced bits count as part of the keys' error.
+// instructions per comparison, and a round of the selection is one redux.max, a ballot and the
+// winner's next key from shared memory.  The replaced bits count as part of the keys' error.
 //
 // A row in doubt ranks its picks, and the few experts that may belong among them, by f64
 // keys, one per lane; only where more than 32 are in doubt are the choices made again one by
-// one (measured: with all rows in doubt made again, 16384 x 256 took 19.8 us for 16.6).
+// one (measured: with all rows in doubt made again, 16384 x 256 took 19.8 us, and 16.6 so).
 //
-// Bound by instruction issue for many tokens (16384 x 256 in 8 groups, top 8: 16.6 us, about
-// 800 instructions a row) and by launch and latency for few (1 x 256: 2.9 us); the bytes (E
-// logits in, 12 k out) are small beside both.
+// Bound by the integer pipe for many tokens (16384 x 256 in 8 groups, top 8: 15.1 us,
+// 780 instructions a row, 340 of them there) and by launch and latency for few (1 x 256: 2.6 us); the bytes
+// (E logits in, 12 k out) are small beside both.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
     constexpr uint32_t kAll = 0xffffffffu;
     constexpr bool kSorted = kPerLane <= 16;
     constexpr uint32_t kPlace = kPerLane - 1u;        // bits of a key that hold the place; kPerLane is a power of two
-    __shared__ uint2 round_picks[kRouteWarps][32];
+    __shared__ uint32_t lists[kRouteWarps][kSorted ? kPerLane - 1 : 1][32], ranked[kRouteWarps][32];
     const uint32_t lane = threadIdx.x & 31;
     const uint32_t t = blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
     ptx::launch_dependents();
@@ -348,45 +348,58 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
             eligible = group_rank_f64<T>(p, row, first, n, group, stats.top, by_sum) < p.topk_groups;
     }
 
+    // The lane's keys.  A lane outside the best groups adds -inf; fmaxf makes NaN -inf; + 0 makes -0 +0.
     uint32_t list[kPerLane];
+    const float in_group = eligible ? 0.f : -INFINITY;
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i)
-        list[i] = eligible && value[i] > -INFINITY ? (order_f32(value[i]) & ~kPlace) | (kPlace - uint32_t(i)) : 0u;
-    if constexpr (kSorted) sort_descending(list);
-    uint2* const picks = round_picks[threadIdx.x >> 5];
-    const uint32_t lower_lanes = (1u << lane) - 1u;
+        list[i] = (order_f32(fmaxf(value[i] + in_group, -INFINITY)) & ~kPlace) | (kPlace - uint32_t(i));
+    // Up to 16 experts are sorted.  The two best are in registers, what follows in shared
+    // memory: a choice then moves one key up, whatever the list's length.
+    uint32_t best = list[0], second = 0, down = 0;    // down: where the next key lies
+    if constexpr (kSorted) {
+        sort_descending(list);
+        best = list[0];
+        second = list[1];
+        uint32_t* const rest = &lists[threadIdx.x >> 5][0][lane];
+#pragma unroll
+        for (int i = 2; i < kPerLane; ++i) rest[(i - 2) * 32] = list[i];
+        rest[(kPerLane - 2) * 32] = 0;                // below every key, for whoever asks further
+    }
     auto lane_best = [&]() {
-        uint32_t best = list[0];
         if constexpr (!kSorted) {
+            best = list[0];
 #pragma unroll
             for (int i = 1; i < kPerLane; ++i) best = max(best, list[i]);
         }
         return best;
     };
-    // A round: the lane with the largest key (of equal ones, the lower lane has the lower
-    // expert) writes it to a pick and passes on to its next.
-    auto round = [&](uint32_t pick, uint32_t m, uint32_t best) {
-        const bool alike = (best | kPlace) == m;
-        const uint32_t all_alike = __ballot_sync(kAll, alike);         // by every lane: not inside a condition
-        const bool won = alike && (all_alike & lower_lanes) == 0;
-        if (won) picks[pick] = make_uint2(best, lane);
+    constexpr uint32_t kNone = 0x007fffffu;           // order_f32(-inf), whose low bits are all set
+    uint2 pick = make_uint2(0u, 0u);                  // lane j: the j-th choice's key and its lane
+    // A round: the lane with the largest key m (of equal ones, the lower lane has the lower
+    // expert) gives it to lane `place` and passes on to its next.
+    auto round = [&](uint32_t place, uint32_t m) {
+        const uint32_t winner = __ffs(__ballot_sync(kAll, (best | kPlace) == m)) - 1;
+        const uint32_t key = __shfl_sync(kAll, best, winner);
+        if (lane == place) pick = make_uint2(key, winner);
         if constexpr (kSorted) {
-#pragma unroll
-            for (int i = 0; i + 1 < kPerLane; ++i) list[i] = won ? list[i + 1] : list[i];
-            list[kPerLane - 1] = won ? 0u : list[kPerLane - 1];
+            if (lane == winner) {
+                best = second;
+                second = lists[threadIdx.x >> 5][down][lane];
+                down = min(down + 1, uint32_t(kPerLane - 2));
+            }
         } else {
 #pragma unroll
-            for (int i = 0; i < kPerLane; ++i) list[i] = won && list[i] == best ? 0u : list[i];
+            for (int i = 0; i < kPerLane; ++i) list[i] = lane == winner && list[i] == key ? 0u : list[i];
         }
     };
-    uint32_t count = 0;                               // picks made
+    uint32_t count = 0;                               // choices made
     uint32_t m = __reduce_max_sync(kAll, lane_best() | kPlace);
-    while (count < p.topk && m != kPlace) {           // kPlace: nothing is left
-        round(count++, m, lane_best());
+    while (count < p.topk && m > kNone) {
+        round(count++, m);
         m = __reduce_max_sync(kAll, lane_best() | kPlace);
     }
-    const uint32_t last = m == kPlace ? 0u : m;       // the best key that is left
-    __syncwarp();
+    const uint32_t last = m > kNone ? m : 0u;         // the best key that is left
     auto order_in_doubt = [&](uint32_t a, uint32_t b) {
         return keyed ? in_doubt(a, b, kPlace, score_error) : !kShort && (a ^ b) <= kPlace;
     };
@@ -394,7 +407,6 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
         return (pick.y >> p.lanes_log2) * p.group_size + (pick.y & ((1u << p.lanes_log2) - 1u)) * p.per_lane + kPlace -
                (pick.x & kPlace);
     };
-    uint2 pick = lane < count ? picks[lane] : make_uint2(0u, 0u);
     const uint32_t after = __shfl_down_sync(kAll, pick.x, 1);
     int chosen = lane < count ? int(expert_of(pick)) : -1;
     if (__any_sync(kAll, lane < count && order_in_doubt(pick.x, lane + 1 == p.topk ? last : after))) {
@@ -402,13 +414,12 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
         const double sum = keyed && !p.sigmoid ? row_sum_f64<T>(p, row, first, n, stats.top) : 1.0;
         const uint32_t border = __shfl_sync(kAll, pick.x, p.topk - 1);   // the last pick, if there are that many
         bool many = false;
-        while (count >= p.topk && m != kPlace && order_in_doubt(border, m)) {
+        while (count >= p.topk && m > kNone && order_in_doubt(border, m)) {
             many = count == 32;
             if (many) break;
-            round(count++, m, lane_best());
+            round(count++, m);
             m = __reduce_max_sync(kAll, lane_best() | kPlace);
         }
-        __syncwarp();
         if (many) {
             chosen = choose_f64<T>(p, row, first, n, eligible, stats.top, sum);
         } else {
@@ -416,7 +427,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
             uint32_t e = 0xffffffffu;
             if (lane < count) {
                 float l, b;
-                e = expert_of(picks[lane]);
+                e = expert_of(pick);
                 load_logit<T>(p, row, e, l, b);
                 key = choice_key(p, stats.top, sum, l, b);
             }
@@ -426,10 +437,10 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
                 const uint32_t other = __shfl_sync(kAll, e, o);
                 rank += k > key || (k == key && other < e);
             }
+            uint32_t* const order = ranked[threadIdx.x >> 5];
+            if (lane < count) order[rank] = e;
             __syncwarp();
-            if (lane < count) picks[rank].x = e;
-            __syncwarp();
-            chosen = lane < min(count, p.topk) ? int(picks[lane].x) : -1;
+            chosen = lane < min(count, p.topk) ? int(order[lane]) : -1;
         }
     }
 
