@@ -10,12 +10,12 @@
 // The mean runs over the unrounded f32 sum h, not over the copy that is written back.
 //
 // Bound by HBM for many rows (9 + 1/32 bytes per element with a BF16 residual and both
-// outputs: 4096 x 7168 in 42.6 us, 6.2 TB/s, 95% of a copy's rate), by launch and load latency
+// outputs: 4096 x 7168 in 42.5 us, 6.2 TB/s, 96% of a copy's rate), by launch and load latency
 // for few (1 x 7168: 2.5 us, where an empty launch takes 2).  One CTA per row keeps the row in
 // registers between the reduction and the output, so every input is read once; a thread holds
-// kChunks x 8 consecutive channels, four lanes share one scale, sixteen one scale word.  With
-// up to 512 threads a row of 7168 needs 32 registers a thread, and four CTAs fit an SM: with
-// two (more registers) the same rows took 48 us.
+// kChunks x 8 consecutive channels, four lanes share one scale, sixteen one scale word.  Up to
+// rows of 8192 a thread has at most 16 channels and 32 registers, and four CTAs fit an SM:
+// with two, for more registers, the same rows took 48 us.
 //
 // A group whose amax lies within f32's rounding of a border, 448 times a power of two, gets
 // one of the two scales next to it; either holds the group.
@@ -67,7 +67,7 @@ __device__ __forceinline__ uint4 pack_bf16x8(const float (&v)[8]) {
 }
 
 template <int kChunks, int kResidual, bool kWeightF32>
-__global__ void __launch_bounds__(kNormThreads) rms_norm_kernel(const NormParams p) {
+__global__ void __launch_bounds__(kNormThreads, kChunks <= 2 ? 4 : 1) rms_norm_kernel(const NormParams p) {
     __shared__ float warp_sums[kNormThreads / 32];
     const uint32_t t = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t chunks = p.hidden / 8;
