@@ -215,7 +215,7 @@ PyObject* route(PyObject*, PyObject* const* args, Py_ssize_t count) {
         a.bias = address(*bias);
     }
     at::Tensor idx, weights;
-    if (args[9] == Py_None) {
+    if (args[9] == Py_None && args[10] == Py_None) {
         idx = new_rows(tokens, topk, at::kLong, *logits);
         weights = new_rows(tokens, topk, at::kFloat, *logits);
     } else {

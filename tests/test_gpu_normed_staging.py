@@ -193,6 +193,37 @@ print('captured')
     assert got.returncode == 0 and 'captured' in got.stdout, got.stderr[-2000:]
 
 
+def test_capture_with_two_streams_that_join():
+    """Norm and product of one half of a batch on a side stream, of the other on the capturing one; routing after both."""
+    x, w, r = (t.cuda() for t in norm_inputs(200, 1024, torch.bfloat16, torch.bfloat16, seed=95))
+    planes = G.transform_router_weight_for_gc_moe(torch.randn((64, 1024), device='cuda') * 0.03)
+    logits = torch.zeros((200, 64), device='cuda')
+
+    def half(rows):
+        return G.router_logits_for_gc_moe(G.rms_norm_for_gc_moe(x[rows], w, r[rows]).normed, planes, out=logits[rows])
+
+    def both(main, side):
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            half(slice(0, 100))
+        half(slice(100, 200))
+        main.wait_stream(side)
+        return G.route_for_gc_moe(logits, 4, scoring='sigmoid')
+
+    main, side = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(main):
+        want = [t.clone() for t in both(main, side)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=main):
+        got = both(main, side)
+    for _ in range(5):
+        logits.fill_(float('nan'))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
 def test_offsets_past_32_bits():
     """Rows 2^29 + 8 elements apart: the last ones start past 2^32 elements."""
     rows, stride = 12, 2 ** 29 + 8

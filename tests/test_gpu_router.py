@@ -300,6 +300,7 @@ def test_no_tokens_and_routing_argument_errors():
                 lambda: call(logits, 8, num_groups=16, topk_groups=1), lambda: call(logits, 8, bias=torch.zeros(64)),
                 lambda: call(logits, 8, bias=torch.zeros(63, device='cuda')), lambda: call(logits, 8, scale=INF),
                 lambda: call(logits, 8, out=(good[0].int(), good[1])), lambda: call(logits, 8, out=(good[0], good[1][:3])),
-                lambda: call(logits, 7, out=good)):
+                lambda: call(logits, 7, out=good), lambda: call(logits, 8, out=(None, good[1])),
+                lambda: call(logits, 8, out=(good[0], None)), lambda: call(None, 8), lambda: call(logits, 8, bias=[0.0] * 64)):
         with pytest.raises(ValueError):
             bad()
