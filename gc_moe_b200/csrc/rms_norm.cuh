@@ -71,8 +71,8 @@ __global__ void __launch_bounds__(kNormThreads, kChunks <= 2 ? 4 : 1) rms_norm_k
     __shared__ float warp_sums[kNormThreads / 32];
     const uint32_t t = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t chunks = p.hidden / 8;
-    ptx::launch_dependents();
     ptx::grid_dependency_wait();
+    ptx::launch_dependents();     // before the wait, later launches crowd in: 256 x 4096 took 2.8 us instead of 2.3
 
     float h[kChunks][8];
     const __nv_bfloat16* row = p.x + t * p.x_stride;
