@@ -220,8 +220,10 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
         *abort_word = 0;
         ptx::fence_mbar_init();
     }
-    __syncwarp();
     __syncthreads();
+    // The first phase of the cluster's barrier ends before anyone writes to another CTA: by
+    // then all of them have started and, where the parts lie in the stages, are done with them.
+    if constexpr (Tile::kApart) ptx::cluster_arrive_relaxed();
     ptx::grid_dependency_wait();
     ptx::launch_dependents();
 
@@ -286,7 +288,7 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
 #pragma unroll
                 for (uint32_t j = 0; j < kBlocks; ++j)
                     ptx::mma_bf16_k64(tmem + which * Tile::kTmemStride, a_desc + at + j * (x_block >> 4),
-                                             b_desc + at + j * (Tile::kColumns * 128 >> 4), idesc, step + j != 0);
+                                      b_desc + at + j * (Tile::kColumns * 128 >> 4), idesc, step + j != 0);
                 ptx::tc_commit<false>(bar_empty + 8 * stage);
                 if (++step == Tile::kChainStages || i == count - 1) {
                     ptx::tc_commit<false>(bar_acc_full + 8 * which);
@@ -341,10 +343,9 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
     __syncthreads();
     // Every load has been consumed and every MMA has ended (the last chain's barrier), or has
     // been drained above.  Row r of the tile belongs to rank r % split, at place r / split of
-    // its part for each sender.  Where the parts lie in the stages, every CTA of the cluster
-    // has told that it is done with them: its loading and MMA warps at their end, the others
-    // when the last chain was complete.
-    if constexpr (!Tile::kApart) ptx::cluster_wait();
+    // its part for each sender.  (Where the parts lie in the stages, the loading and MMA warps
+    // have arrived at their end, the others when the last chain was complete.)
+    ptx::cluster_wait();
     const uint32_t part = base + Tile::kPartOffset, owned = kM / p.split;
     if (warp >= 2 && warp < 10) {
         const bool failed = *abort_word != 0u;
@@ -352,11 +353,12 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
         const uint32_t side = (warp - 2) >> 2, token = kM == 128 ? (warp & 3) * 32 + lane : (warp & 3) * 16 + (lane & 15);
         const uint32_t at = part + ((rank * owned + token / p.split) * Tile::kPitch + side * (kN / 2)) * 4;
         const uint32_t to = ptx::mapa(at, token % p.split);
-        if (kM == 128 || lane < 16)
+        if (kM == 128 || lane < 16) {
 #pragma unroll
-        for (int j = 0; j < kN / 2; j += 4)
-            ptx::st_cluster_f32x4(to + j * 4, failed ? make_float4(NAN, NAN, NAN, NAN)
-                                                     : make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]));
+            for (int j = 0; j < kN / 2; j += 4)
+                ptx::st_cluster_f32x4(to + j * 4, failed ? make_float4(NAN, NAN, NAN, NAN)
+                                                         : make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]));
+        }
     } else if (warp == 1) {
         ptx::tc_fence_after();
         ptx::tmem_dealloc<false>(tmem, Tile::kTmemColumns);
