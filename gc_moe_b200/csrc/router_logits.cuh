@@ -127,9 +127,9 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_fma_kernel(const __grid
 // registers, rounded to nearest; two accumulators in TMEM keep the MMAs going meanwhile.
 //
 // Bound by launch, load latency and the partial tiles' exchange for up to a few hundred
-// tokens (33 x 5120 x 384: 4.1 us, of which an empty launch takes 2), then by the MMAs (82
+// tokens (33 x 5120 x 384: 4.2 us, of which an empty launch takes 2), then by the MMAs (82
 // cycles for 128 x 128, 64 at best) and the traffic from L2 to the SMs: 4096 x 7168 x 256 takes
-// 18.8 us with 235 MB brought to the SMs; the inputs need 10.2 us of HBM.  Tiles of 256
+// 18.7 us with 235 MB brought to the SMs; the inputs need 10.2 us of HBM.  Tiles of 256
 // experts, as one CTA or as a pair with 256 tokens, move half to two thirds of that but were
 // no faster at any size (20.8 and 22 us here): their shared memory holds too few stages to
 // cover the latency.  An MMA of 64 rows takes half the time of one of 128, and its smaller

@@ -41,7 +41,8 @@ def rms_norm_for_gc_moe(x: torch.Tensor, weight: torch.Tensor, residual: Optiona
     write it to), and ``h`` in the type of ``residual``: in ``residual_out``,
     which may be ``residual`` itself, or a new tensor.  Rows may have a stride;
     their starts are 16-byte aligned.  Apart from ``residual_out`` being
-    ``residual``, outputs overlap no input.
+    ``residual``, outputs overlap no input.  The squares are summed in FP32: rows
+    whose sum overflows it (entries beyond 1e17) do not come out as the formula says.
 
     Runs on the current stream and can be captured.
     """
