@@ -812,10 +812,47 @@ extern "C" int gcmoe_rms_norm(const gcmoe_norm_args* args, void* cuda_stream) {
     return GCMOE_OK;
 }
 
-template <int kTokens, int kPlanes>
-static cudaError_t launch_logits_fma(const LogitsParams& p, cudaStream_t s) {
+using LogitsFmaKernel = void (*)(const LogitsParams);
+struct LogitsFmaForm {
+    LogitsFmaKernel kernel;       // null: the tensor-core form
+    uint32_t tokens;              // of a CTA
+};
+
+// The FMA form: the fewest tokens a CTA (1, 2, 4) whose CTAs are all resident at once, and the
+// tensor cores where even four tokens a CTA are too many.  Measured, us, H x E x tokens.  One
+// plane: 7168 x 256 x 1 with 1 and 4 rounds 2.1 and 2.7; 7168 x 256 x 8 with 2 and 4 tokens a
+// CTA 3.6 and 4.3, on the tensor cores 4.4; 5120 x 384 x 8 (768 CTAs of 2 tokens) 4.2 and 3.7,
+// tensor cores 4.2; 7168 x 512 x 8 (512 CTAs of 4) 5.4, tensor cores 5.0.
+// Three planes, two tokens a CTA also for one token: 7168 x 256 x 4 with 2 and 4 tokens a CTA
+// 3.4 and 4.0, tensor cores 4.8; 5120 x 384 x 8 (384 CTAs of 4) 5.7, tensor cores 4.6; one or
+// two tokens stay here for any E (4096 x 1024 x 1 4.3, tensor cores 5.4; worst 2048 x 2048 x 1,
+// 6.5 and 5.8).  Two rounds cover a row of 512 chunks, four one of 1024: 4096 x 256 x 8 3.0 and
+// 4.1, 7168 x 256 x 8 4.5 and 4.2; longer rows are no faster here (16384 x 256 x 4: 7.5 and 7.4).
+static LogitsFmaForm logits_fma_form(const gcmoe_logits_args& a, bool forced) {
+    const uint32_t pairs = (a.num_experts + 1) / 2;
+    auto fits = [&](uint32_t tokens, uint32_t resident) {
+        return uint64_t(pairs) * ((a.num_tokens + tokens - 1) / tokens) <= uint64_t(resident) * 148;
+    };
+    if (a.planes == 1) {
+        if (a.num_tokens == 1) return {logits_fma_kernel<1, 1, 1>, 1};
+        if (fits(2, kFmaResident<2, 1>)) return {logits_fma_kernel<2, 1, 2>, 2};
+        if (forced || fits(4, kFmaResident<4, 1>)) return {logits_fma_kernel<4, 1, 2>, 4};
+        return {nullptr, 0};
+    }
+    const uint32_t chunks = a.hidden / 8;
+    if (chunks <= 2 * kLogitsThreads) {
+        if (a.num_tokens <= 2 || fits(2, kFmaResident<2, 3>)) return {logits_fma_kernel<2, 3, 2>, 2};
+        if (forced || fits(4, kFmaResident<4, 3>)) return {logits_fma_kernel<4, 3, 2>, 4};
+    } else if (forced || chunks <= 4 * kLogitsThreads) {
+        if (a.num_tokens <= 2 || fits(2, kFmaResident<2, 3>)) return {logits_fma_kernel<2, 3, 4>, 2};
+        if (forced || fits(4, kFmaResident<4, 3>)) return {logits_fma_kernel<4, 3, 4>, 4};
+    }
+    return {nullptr, 0};
+}
+
+static cudaError_t launch_logits_fma(const LogitsFmaForm& form, const LogitsParams& p, cudaStream_t s) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((p.num_experts + 1) / 2, (p.num_tokens + kTokens - 1) / kTokens);
+    cfg.gridDim = dim3((p.num_experts + 1) / 2, (p.num_tokens + form.tokens - 1) / form.tokens);
     cfg.blockDim = dim3(kLogitsThreads);
     cfg.stream = s;
     cudaLaunchAttribute attr;
@@ -823,7 +860,7 @@ static cudaError_t launch_logits_fma(const LogitsParams& p, cudaStream_t s) {
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, logits_fma_kernel<kTokens, kPlanes>, p);
+    return cudaLaunchKernelEx(&cfg, form.kernel, p);
 }
 
 // Tile and split of the tensor-core form: the choice with the least estimated time, in
@@ -923,15 +960,13 @@ extern "C" int gcmoe_router_logits(const gcmoe_logits_args* args, void* cuda_str
     p.num_tokens = a.num_tokens; p.num_experts = a.num_experts; p.hidden = a.hidden;
     cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
     // Rows that overlap (a broadcast row) have no tensor map.
-    if (a.num_tokens <= kFmaMaxTokens || a.x_stride < a.hidden || a.x_stride >= (1ull << 39)) {
-        auto by_tokens = [&](auto planes) {
-            constexpr int kPlanes = decltype(planes)::value;
-            return p.num_tokens == 1   ? launch_logits_fma<1, kPlanes>(p, s)
-                   : p.num_tokens == 2 ? launch_logits_fma<2, kPlanes>(p, s)
-                                       : launch_logits_fma<4, kPlanes>(p, s);
-        };
-        GCMOE_CUDA(a.planes == 1 ? by_tokens(std::integral_constant<int, 1>()) : by_tokens(std::integral_constant<int, 3>()));
-        return GCMOE_OK;
+    const bool forced = a.x_stride < a.hidden || a.x_stride >= (1ull << 39);
+    if (forced || a.num_tokens <= kFmaMaxTokens) {
+        const LogitsFmaForm form = logits_fma_form(a, forced);
+        if (form.kernel != nullptr) {
+            GCMOE_CUDA(launch_logits_fma(form, p, s));
+            return GCMOE_OK;
+        }
     }
     const LogitsPlan plan = plan_logits(a.num_tokens, a.num_experts, a.hidden, a.planes);
     if (plan.tokens == 64) {

@@ -28,16 +28,20 @@ struct LogitsParams {
     uint32_t num_tokens, num_experts, hidden;
 };
 
-// Few tokens: bound by the latency of the loads, so a thread has the loads of several
-// rounds of the loop in flight.  Measured (H 7168, E 256), us for 1, 4, 8 and 16 tokens:
-// BF16 weight 2.6, 3.8, 4.1, 5.2 in this form, 4.3, 4.3, 4.3, 4.3 on the tensor cores; FP32
-// weight 4.3, 4.3, 4.5, 8.0 and 4.8, 4.8, 4.8, 4.9.
+// Few tokens: bound by the latency of the loads, so a thread has the loads of kRounds rounds
+// of the loop in flight, and all CTAs should be resident at once.  A thread adds its channels
+// in the same order in every variant.  The launch chooses one; with nine tokens, in four and
+// on the tensor cores: 5120 x 384 5.1 and 4.2 us, FP32 weight 7.3 and 4.6; 4096 x 64 3.4 and 3.5.
 constexpr uint32_t kFmaMaxTokens = 8;
 
+// CTAs of an SM, the least that the compiler has to leave registers for.
 template <int kTokens, int kPlanes>
-__global__ void __launch_bounds__(kLogitsThreads) logits_fma_kernel(const __grid_constant__ LogitsParams p) {
+constexpr uint32_t kFmaResident = kPlanes == 3 ? 2 : kTokens <= 2 ? 4 : 3;
+
+template <int kTokens, int kPlanes, int kRounds>
+__global__ void __launch_bounds__(kLogitsThreads, kFmaResident<kTokens, kPlanes>)
+    logits_fma_kernel(const __grid_constant__ LogitsParams p) {
     constexpr int kExperts = 2, kSums = kTokens * kExperts;
-    constexpr int kRounds = kPlanes == 1 ? 4 : 2;             // rounds of loads in flight
     __shared__ float partial[kLogitsThreads / 32][kSums];
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t e0 = blockIdx.x * kExperts, t0 = blockIdx.y * kTokens;
@@ -127,7 +131,7 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_fma_kernel(const __grid
 // registers, rounded to nearest; two accumulators in TMEM keep the MMAs going meanwhile.
 //
 // Bound by launch, load latency and the partial tiles' exchange for up to a few hundred
-// tokens (33 x 5120 x 384: 4.2 us, of which an empty launch takes 2), then by the MMAs (82
+// tokens (33 x 5120 x 384: 4.2 us, an empty launch 0.6), then by the MMAs (82
 // cycles for 128 x 128, 64 at best) and the traffic from L2 to the SMs: 4096 x 7168 x 256 takes
 // 18.7 us with 235 MB brought to the SMs; the inputs need 10.2 us of HBM.  Tiles of 256
 // experts, as one CTA or as a pair with 256 tokens, move half to two thirds of that but were

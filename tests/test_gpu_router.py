@@ -52,6 +52,24 @@ def test_logits_against_the_formula(tokens, hidden, experts, weight):
     assert torch.equal(got, G.router_logits_for_gc_moe(x.cuda(), planes))      # the same bits every time
 
 
+# Few tokens: rows of one, two and four rounds of loads and longer ones, and as many experts as are
+# computed with one, two and four tokens at a time, and more.
+@pytest.mark.parametrize('weight', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('hidden,experts', [
+    (2048, 129), (4096, 256), (4104, 296), (4104, 297), (5120, 384), (5120, 385), (8192, 592), (8200, 593), (16384, 64),
+    (1032, 888), (1032, 889), (520, 2048), (8, 2047)])
+def test_logits_of_few_tokens(hidden, experts, weight):
+    x, w = _logits_case(8, hidden, experts, weight, seed=hidden + experts)
+    planes = G.transform_router_weight_for_gc_moe(w.cuda())
+    for tokens in range(1, 9):
+        guard = torch.full((tokens + 2, experts), 7.0, device='cuda')
+        got = G.router_logits_for_gc_moe(x[:tokens].cuda(), planes, out=guard[1:-1])
+        _check_logits(got, x[:tokens], w)
+        assert bool((guard[0] == 7).all()) and bool((guard[-1] == 7).all())
+        same = G.router_logits_for_gc_moe(x[:1].cuda().expand(tokens, hidden), planes)     # rows that overlap
+        _check_logits(same, x[:1].expand(tokens, hidden), w)
+
+
 @pytest.mark.parametrize('tokens', [1, 5, 40, 300])
 def test_logits_of_strided_rows_into_a_given_tensor(tokens):
     x, w = _logits_case(tokens, 1024, 100, torch.bfloat16, seed=tokens)
