@@ -794,8 +794,15 @@ extern "C" int gcmoe_rms_norm(const gcmoe_norm_args* args, void* cuda_stream) {
     p.shared_sf_rows = a.shared_sf_rows; p.block_m = a.block_m;
     p.hidden = a.hidden; p.eps = a.eps;
     const uint32_t chunks = a.hidden / 8;
-    uint32_t per_thread = 1;
-    while (per_thread * kNormThreads < chunks) per_thread *= 2;
+    // The longest row, in 8-channel chunks, that gets a thread for each chunk.  Up to one row an
+    // SM the latency counts: with at most 1024 and 512 threads 64 x 5120 takes 2.1 and 2.5 us,
+    // 148 x 7168 2.6 and 2.8; but with two rows an SM 256 x 5120 takes 3.6 and 3.1.  From some
+    // 1024 rows on two chunks a thread, for fewer threads to reduce over: 1024 x 2048 3.5 us,
+    // with one 3.8; 4096 x 4096 25.3 and 26.3; the last wave's fill can outweigh it (1500 x 2048:
+    // 6.3 and 5.6, 1024 x 2560: 5.6 and 5.0).  They gain nothing on 4096 x 1024, 6.7 us either way.
+    const uint32_t single = a.num_tokens <= 148 ? kNormThreads : a.num_tokens < 1024 ? kNormThreads / 2 : 128;
+    // Rows above 1024 chunks: four a thread, 512 to 1024 threads (4096 x 16384: 93 us).
+    const uint32_t per_thread = chunks <= single ? 1 : chunks <= kNormThreads ? 2 : 4;
     const uint32_t threads = round_up_u32((chunks + per_thread - 1) / per_thread, 32);
     const int residual = a.residual == 0 ? kNoResidual : a.residual_f32 ? kResidualF32 : kResidualBf16;
     cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
@@ -805,10 +812,9 @@ extern "C" int gcmoe_rms_norm(const gcmoe_norm_args* args, void* cuda_stream) {
              : residual == kResidualBf16 ? launch_norm<kChunks, kResidualBf16>(a, p, threads, s)
                                          : launch_norm<kChunks, kResidualF32>(a, p, threads, s);
     };
-    GCMOE_CUDA(per_thread == 1 ? by_residual(std::integral_constant<int, 1>())
+    GCMOE_CUDA(per_thread == 1   ? by_residual(std::integral_constant<int, 1>())
                : per_thread == 2 ? by_residual(std::integral_constant<int, 2>())
-               : per_thread == 4 ? by_residual(std::integral_constant<int, 4>())
-                                 : by_residual(std::integral_constant<int, 8>()));
+                                 : by_residual(std::integral_constant<int, 4>()));
     return GCMOE_OK;
 }
 

@@ -10,12 +10,12 @@
 // The mean runs over the unrounded f32 sum h, not over the copy that is written back.
 //
 // Bound by HBM for many rows (9 + 1/32 bytes per element with a BF16 residual and both
-// outputs: 4096 x 7168 in 42.5 us, 6.2 TB/s, 96% of a copy's rate), by launch and load latency
-// for few (1 x 7168: 2.5 us, where an empty launch takes 2).  One CTA per row keeps the row in
-// registers between the reduction and the output, so every input is read once; a thread holds
-// kChunks x 8 consecutive channels, four lanes share one scale, sixteen one scale word.  Up to
-// rows of 8192 a thread has at most 16 channels and 32 registers, and four CTAs fit an SM:
-// with two, for more registers, the same rows took 48 us.
+// outputs: 4096 x 7168 in 42.5 us, 6.2 TB/s, 96% of a copy's rate), by load latency
+// and the reduction for few (1 x 7168: 2.4 us, an empty launch 0.6).  One CTA per row keeps the
+// row in registers between the reduction and the output, so every input is read once; a thread
+// holds kChunks times 8 channels, four lanes share one scale, sixteen one scale word.
+// Up to 16 channels a thread take 32 registers, so that 2048 threads fit an SM: with more
+// registers and half of the rows in flight, 4096 x 7168 took 48 us.
 //
 // A group whose amax lies within f32's rounding of a border, 448 times a power of two, gets
 // one of the two scales next to it; either holds the group.
@@ -31,8 +31,8 @@
 
 namespace gcmoe {
 
-constexpr uint32_t kNormThreads = 512;       // most threads of a CTA
-constexpr uint32_t kNormMaxChunks = 8;       // most 8-channel chunks of a thread
+constexpr uint32_t kNormThreads = 1024;      // most threads of a CTA
+constexpr uint32_t kNormMaxChunks = 4;       // most 8-channel chunks of a thread
 enum NormResidual : int { kNoResidual = 0, kResidualBf16 = 1, kResidualF32 = 2 };
 
 struct NormParams {
@@ -67,8 +67,8 @@ __device__ __forceinline__ uint4 pack_bf16x8(const float (&v)[8]) {
 }
 
 template <int kChunks, int kResidual, bool kWeightF32>
-__global__ void __launch_bounds__(kNormThreads, kChunks <= 2 ? 4 : 1) rms_norm_kernel(const NormParams p) {
-    __shared__ float warp_sums[kNormThreads / 32];
+__global__ void __launch_bounds__(kNormThreads, kChunks <= 2 ? 2 : 1) rms_norm_kernel(const NormParams p) {
+    __shared__ float group_sums[kNormThreads / 32 * kChunks];      // a group: 32 consecutive chunks
     const uint32_t t = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t chunks = p.hidden / 8;
     ptx::grid_dependency_wait();
@@ -128,23 +128,34 @@ __global__ void __launch_bounds__(kNormThreads, kChunks <= 2 ? 4 : 1) rms_norm_k
         }
     }
 
-    float sum = 0.f;
+    // The order of the additions depends on the row's length alone, not on the threads that
+    // share the row: a row has the same bits in a batch of any size.  With several chunks a
+    // thread that takes a shuffle for each (511 x 7168: 6.0 us instead of 5.9).
+    float sum[kChunks];
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
-        float part = 0.f;
+        sum[i] = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) part = fmaf(h[i][j], h[i][j], part);
-        sum += part;
+        for (int j = 0; j < 8; ++j) sum[i] = fmaf(h[i][j], h[i][j], sum[i]);
     }
 #pragma unroll
-    for (uint32_t d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if (lane == 0) warp_sums[warp] = sum;
-    __syncthreads();
-    // every warp adds the warps' sums in the same order
-    float total = lane < blockDim.x / 32 ? warp_sums[lane] : 0.f;
+    for (uint32_t d = 16; d > 0; d >>= 1)
 #pragma unroll
-    for (uint32_t d = 8; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
-    total = __shfl_sync(0xffffffffu, total, 0);
+        for (int i = 0; i < kChunks; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], d);
+    if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) group_sums[warp + i * (blockDim.x / 32)] = sum[i];
+    }
+    __syncthreads();
+    // the CTA's warps hold all of the row's groups; up to two chunks a thread there are at most 32
+    const uint32_t groups = (chunks + 31) / 32;
+    float total = lane < groups ? group_sums[lane] : 0.f;
+    if constexpr (kChunks > 2) {
+#pragma unroll
+        for (uint32_t g = 32; g < kNormThreads / 32 * kChunks; g += 32) total += lane + g < groups ? group_sums[lane + g] : 0.f;
+    }
+#pragma unroll
+    for (uint32_t d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
     const float scale = 1.0f / sqrtf(total / float(p.hidden) + p.eps);
 
     uint32_t shared_row = 0;

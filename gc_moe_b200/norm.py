@@ -43,6 +43,7 @@ def rms_norm_for_gc_moe(x: torch.Tensor, weight: torch.Tensor, residual: Optiona
     their starts are 16-byte aligned.  Apart from ``residual_out`` being
     ``residual``, outputs overlap no input.  The squares are summed in FP32: rows
     whose sum overflows it (entries beyond 1e17) do not come out as the formula says.
+    A row's result does not depend on the other rows or their number.
 
     Runs on the current stream and can be captured.
     """

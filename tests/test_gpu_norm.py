@@ -83,6 +83,21 @@ def test_against_the_formula(tokens, hidden, residual, weight):
     assert torch.equal(only.x.view(torch.uint8), got.x.view(torch.uint8)) and torch.equal(only.x_sf, got.x_sf)
 
 
+@pytest.mark.parametrize('residual', [None, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('hidden', [1024, 1056, 2560, 4096, 4128, 8192, 8224, 16416, 32768])
+def test_a_row_has_the_same_bits_in_a_batch_of_any_size(hidden, residual):
+    x, w, r = _inputs(3, hidden, residual, torch.bfloat16, seed=hidden)
+    x, w, r = x.cuda(), w.cuda(), None if r is None else r.cuda()
+    one = G.rms_norm_for_gc_moe(x, w, r)
+    _check(one, x.cpu(), w.cpu(), None if r is None else r.cpu(), 1e-6)
+    for tokens in (148, 149, 1023, 1024):
+        rows = torch.arange(tokens, device='cuda') % 3
+        got = G.rms_norm_for_gc_moe(x[rows], w, None if r is None else r[rows])
+        assert torch.equal(got.normed, one.normed[rows]) and torch.equal(got.x_sf, one.x_sf[rows])
+        assert torch.equal(got.x.view(torch.uint8), one.x.view(torch.uint8)[rows])
+        assert r is None or torch.equal(got.residual, one.residual[rows])
+
+
 def test_rows_that_exercise_the_scale_rule():
     """Zero rows and groups (scale byte 0 and zeros, no NaN), a row of equal values, one hot channel, tiny and
     large magnitudes."""
