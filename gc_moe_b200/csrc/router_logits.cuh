@@ -157,6 +157,8 @@ struct LogitsTile {
     static constexpr uint32_t kChainStages = kChainBlocks / kStageBlocks;
     // The partial tile that a CTA receives, row by row from every rank: its own memory where
     // that leaves room for enough stages, else the stages' once they are done with.
+    // Apart from the stages, tiles of 128 x 128 take 24.1 us instead of 18.9 (4096 x 7168 x
+    // 256); in the stages' memory, small ones 4.39 instead of 4.23 (33 x 5120 x 384).
     static constexpr uint32_t kPitch = kN + 4;                 // floats per row: no bank conflicts
     static constexpr uint32_t kPartBytes = kM * kPitch * 4;
     static constexpr bool kApart = kN <= 64;
