@@ -373,7 +373,8 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
     // After this no CTA touches another's memory.
     ptx::cluster_sync();
     const uint32_t rows = min(kM, p.num_tokens - t0);
-    const bool vectors = p.num_experts % 4 == 0;
+    // `out` may start at any f32: whole vectors where every row starts on 16 bytes
+    const bool vectors = p.num_experts % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
     for (uint32_t i = tid; i < owned * (kN / 4); i += kLogitsMmaThreads) {
         const uint32_t place = i / (kN / 4), r = place * p.split + rank, c = i % (kN / 4) * 4;
         if (r >= rows || e0 + c >= p.num_experts) continue;

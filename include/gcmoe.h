@@ -217,7 +217,7 @@ int gcmoe_rms_norm(const gcmoe_norm_args* args, void* cuda_stream);
 typedef struct gcmoe_logits_args {
     uint64_t x;               /* bf16 [T, H], rows 16-byte aligned                    */
     uint64_t weight;          /* bf16 [planes, E, H], contiguous, 16-byte aligned     */
-    uint64_t out;             /* out: f32 [T, E], contiguous                          */
+    uint64_t out;             /* out: f32 [T, E], contiguous, at any 4-byte address   */
     uint64_t x_stride;        /* elements between rows of x                           */
     uint32_t num_tokens, hidden, num_experts, planes;
     int32_t device;
