@@ -917,8 +917,11 @@ static int launch_logits_mma(const gcmoe_logits_args& a, uint32_t split, cudaStr
     if (int rc = encode_map(&p.x_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.x, x_dims, &x_pitch, x_box, "router input")) return rc;
     if (int rc = encode_map(&p.w_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.weight, w_dims, &w_pitch, w_box, "router weight"))
         return rc;
+    p.x = reinterpret_cast<const __nv_bfloat16*>(a.x);
+    p.weight = reinterpret_cast<const __nv_bfloat16*>(a.weight);
     p.out = reinterpret_cast<float*>(a.out);
-    p.num_tokens = a.num_tokens; p.num_experts = a.num_experts;
+    p.x_stride = a.x_stride;
+    p.num_tokens = a.num_tokens; p.num_experts = a.num_experts; p.hidden = a.hidden;
     p.k_stages = (a.hidden + kLogitsBlockK * Tile::kStageBlocks - 1) / (kLogitsBlockK * Tile::kStageBlocks);
     p.split = split;                                   // at most half of the K blocks: no CTA is without a stage
     // the attributes are the device's and outlive the call: set once for each

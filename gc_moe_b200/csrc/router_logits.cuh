@@ -176,13 +176,57 @@ struct LogitsTile {
 struct LogitsMmaParams {
     CUtensorMap x_map;            // bf16 [T][H], box 64 x box_tokens, 128-byte swizzle
     CUtensorMap w_map;            // bf16 [P * E][H], box 64 x kN
+    const __nv_bfloat16* x;       // the same memory, for rows with infinities
+    const __nv_bfloat16* weight;
     float* out;                   // [T][E]
-    uint32_t num_tokens, num_experts;
+    uint64_t x_stride;            // elements between rows
+    uint32_t num_tokens, num_experts, hidden;
     uint32_t k_stages;            // stages that cover H; channels past H are filled with zeros
     uint32_t box_tokens;          // rows a load of x brings: fewer than a tile when there are fewer tokens; the rest of
                                   // the tile's rows keep what shared memory held and end in rows that are not stored
     uint32_t split;               // CTAs of a cluster, over which a tile's K blocks are split: 1, 2, 4 or 8
 };
+
+// What a CTA that gave up sends: a NaN that no addition makes (those have all bits set).
+constexpr uint32_t kGaveUpBits = 0x7fc0deadu;
+
+// Four experts' logits of a row whose sums over three planes are not all numbers.  Infinity
+// times a plane that is zero, or times planes of both signs, is NaN although infinity times the
+// weight is an infinity; the FMA form, which adds the planes first, has none of this.  What
+// the formula gives is decided by the row's infinite channels alone.  One thread reads the
+// whole row, which only calls with such a row pay for (33 x 7168 x 256: 0.12 ms with one).
+static __device__ __noinline__ float4 infinite_row_logits(const LogitsMmaParams& p, uint32_t t, uint32_t e, float4 sum) {
+    const uint4* const row = reinterpret_cast<const uint4*>(p.x + t * p.x_stride);
+    const uint64_t plane = uint64_t(p.num_experts) * p.hidden;
+    const uint32_t chunks = p.hidden / 8;
+    float acc[4] = {};
+    bool infinite = false;
+    for (uint32_t c0 = 0; c0 < chunks; c0 += 8) {
+        uint4 raw[8];                                                     // eight loads in flight; past the end the last again
+        bool numbers = true;
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) raw[i] = row[min(c0 + i, chunks - 1)];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            const uint32_t v[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) numbers = numbers && (v[j] & 0x7f80u) != 0x7f80u && (v[j] & 0x7f800000u) != 0x7f800000u;
+        }
+        if (numbers) continue;
+        for (uint32_t k = c0 * 8; k < min(c0 * 8 + 64, p.hidden); ++k) {
+            const float v = __bfloat162float(p.x[t * p.x_stride + k]);
+            if (isnan(v) || (isnan(acc[0]) && isnan(acc[1]) && isnan(acc[2]) && isnan(acc[3])))
+                return make_float4(NAN, NAN, NAN, NAN);
+            if (!isinf(v)) continue;
+            infinite = true;
+            for (uint32_t i = 0; i < 4 && e + i < p.num_experts; ++i) {
+                const __nv_bfloat16* const w = p.weight + uint64_t(e + i) * p.hidden + k;
+                acc[i] = fmaf(v, __bfloat162float(w[0]) + (__bfloat162float(w[plane]) + __bfloat162float(w[2 * plane])), acc[i]);
+            }
+        }
+    }
+    return infinite ? make_float4(acc[0], acc[1], acc[2], acc[3]) : sum;
+}
 
 template <int kM, int kN, int kPlanes>
 __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const __grid_constant__ LogitsMmaParams p) {
@@ -355,6 +399,7 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
     const uint32_t part = base + Tile::kPartOffset, owned = kM / p.split;
     if (warp >= 2 && warp < 10) {
         const bool failed = *abort_word != 0u;
+        const float gave_up = __uint_as_float(kGaveUpBits);
         // an accumulator of 64 rows has 16 of them in the first half of each quarter of the lanes
         const uint32_t side = (warp - 2) >> 2, token = kM == 128 ? (warp & 3) * 32 + lane : (warp & 3) * 16 + (lane & 15);
         const uint32_t at = part + ((rank * owned + token / p.split) * Tile::kPitch + side * (kN / 2)) * 4;
@@ -362,7 +407,7 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
         if (kM == 128 || lane < 16) {
 #pragma unroll
             for (int j = 0; j < kN / 2; j += 4)
-                ptx::st_cluster_f32x4(to + j * 4, failed ? make_float4(NAN, NAN, NAN, NAN)
+                ptx::st_cluster_f32x4(to + j * 4, failed ? make_float4(gave_up, gave_up, gave_up, gave_up)
                                                          : make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]));
         }
     } else if (warp == 1) {
@@ -380,9 +425,15 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
         if (r >= rows || e0 + c >= p.num_experts) continue;
         const float* const from = reinterpret_cast<const float*>(smem + Tile::kPartOffset) + place * Tile::kPitch + c;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        bool complete = true;
         for (uint32_t s = 0; s < p.split; ++s) {                          // in rank order
             const float4 v = *reinterpret_cast<const float4*>(from + s * owned * Tile::kPitch);
+            complete = complete && __float_as_uint(v.x) != kGaveUpBits;
             sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+        }
+        if constexpr (kPlanes == 3) {
+            if (complete && (isnan(sum.x) || isnan(sum.y) || isnan(sum.z) || isnan(sum.w)))
+                sum = infinite_row_logits(p, t0 + r, e0 + c, sum);
         }
         float* const out = p.out + static_cast<uint64_t>(t0 + r) * p.num_experts + e0 + c;
         if (vectors) {

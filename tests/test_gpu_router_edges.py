@@ -12,6 +12,8 @@ import gc_moe_b200 as G
 
 pytestmark = pytest.mark.gpu
 
+INF = float('inf')
+
 
 def _case(tokens, experts, hidden, weight, seed):
     g = torch.Generator().manual_seed(seed)
@@ -41,3 +43,37 @@ def test_logits_into_a_view_at_any_address(tokens, experts, weight):
         assert got.data_ptr() == flat.data_ptr() + 4 * shift
         assert torch.equal(got, want)
         assert bool((flat[:shift] == 7).all()) and bool((flat[shift + size:] == 7).all())
+
+
+@pytest.mark.parametrize('weight', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('tokens,experts,hidden', [(3, 70, 2048), (8, 70, 2048), (9, 70, 2048), (150, 70, 2048), (150, 384, 512),
+                                                   (300, 384, 2048), (1000, 384, 2048), (40, 65, 1000)])
+def test_an_infinity_gives_what_the_formula_gives(tokens, experts, hidden, weight):
+    """Whatever the number of tokens and the weight's planes: an infinite activation times the weight is an infinity of
+    the weight's sign, NaN where the weight is zero or where both infinities meet.  Weights with one, two and three
+    planes that are not zero, and planes of both signs."""
+    x, w = _case(tokens, experts, hidden, weight, seed=tokens)
+    w[:, 5:9] = torch.tensor([1.0, -2.0, 1 + 2.0 ** -10, -(1 + 2.0 ** -10 - 2.0 ** -18)])
+    w[3, 5] = 0.0
+    w[4, 6] = -0.0
+    w[5:9, 11] = torch.tensor([2.0 ** -40, -2.0 ** -40, 1 - 2.0 ** -9, -1 + 2.0 ** -20])
+    x[0, 5] = INF
+    x[1, 6] = -INF
+    x[2, [7, 8]] = INF                                    # infinities of both signs meet
+    if tokens > 3:
+        x[3, [5, 7]] = INF                                # of one sign
+        x[4, 11] = INF
+        x[5, hidden - 1] = -INF
+        x[6, 8], x[6, 9] = INF, float('nan')
+        x[7] = INF
+    rows = min(tokens, 8)
+    got = G.router_logits_for_gc_moe(x.cuda(), G.transform_router_weight_for_gc_moe(w.cuda())).cpu()
+    # element by element: a library product need not keep infinities apart
+    want = (x[:rows, None, :].double() * w[None].double()).sum(-1)
+    special = ~torch.isfinite(want)
+    assert bool(special.any(1).all())
+    assert torch.equal(torch.isnan(got[:rows]), torch.isnan(want))
+    assert torch.equal(got[:rows][special & ~torch.isnan(want)].double(), want[special & ~torch.isnan(want)])
+    assert bool(torch.isfinite(got[rows:]).all())
+    if tokens > rows:
+        assert _close(got[rows:].cuda(), x[rows:], w)
