@@ -112,6 +112,8 @@ class GCSymmBuffer:
         _typed_views(self.buffer, self.layout, self)
         self._plans = {}          # launch plans cached per call signature
         self._retired_scratch = []   # scratch blocks of evicted plans, until their status has been read
+        from . import operator
+        self._producer_failures_seen = operator.producer_failures(self.buffer.device)   # those before this workspace
 
     def _for_call(self, num_shared_experts: int):
         """View of the same bytes laid out for the shared-expert count of one
@@ -148,15 +150,31 @@ class GCSymmBuffer:
 
     def raise_on_device_error(self) -> None:
         """Synchronise and raise RuntimeError if a kernel of any call on this
-        workspace, or of ``router_logits_for_gc_moe`` on its device, gave up on a
-        bounded wait."""
+        workspace gave up on a bounded wait, or one of ``router_logits_for_gc_moe``
+        on the workspace's device: those are not tied to a workspace, so every
+        workspace of the device raises for them, once.  Covers what the current
+        stream of that device is ordered after."""
         from . import operator
-        operator.check_producer_status()
-        for plan in list(self._plans.values()):
-            operator.check_plan_status(plan)
-        retired, self._retired_scratch = self._retired_scratch, []
-        for scratch in retired:       # the status reads above have synchronised the stream
-            operator.check_retired_status(scratch)
+        if self.buffer is None:
+            return                    # destroyed: no plans, no device
+        errors = []
+
+        def collect(check, *args):
+            try:
+                check(*args)
+            except RuntimeError as error:
+                errors.append(str(error))
+
+        device = self.buffer.device
+        with torch.cuda.device(device):
+            for plan in list(self._plans.values()):
+                collect(operator.check_plan_status, plan)
+            retired, self._retired_scratch = self._retired_scratch, []
+            for scratch in retired:       # the status reads above have synchronised the stream
+                collect(operator.check_retired_status, scratch)
+            collect(operator.check_producer_status, self, device)
+        if errors:
+            raise RuntimeError('; '.join(dict.fromkeys(errors)))
 
     def destroy(self):
         from . import operator

@@ -993,16 +993,27 @@ extern "C" int gcmoe_router_logits(const gcmoe_logits_args* args, void* cuda_str
     }
 }
 
+// Reads the status words and clears the code in one step, so that a failure recorded meanwhile
+// by a launch on another stream is either in the report or still there for the next query.
+static __device__ uint32_t g_producer_report[kStatusWords];
+__global__ void take_producer_status_kernel() {
+    g_producer_report[kStatusCode] = atomicExch(&g_producer_status[kStatusCode], 0u);
+    __threadfence();
+    for (int i = 1; i < kStatusWords; ++i) g_producer_report[i] = *const_cast<volatile uint32_t*>(&g_producer_status[i]);
+}
+
 // Status words of the producers' bounded waits after synchronising the stream; a failure is
 // reported once and cleared.
 extern "C" int gcmoe_producer_status(void* cuda_stream, uint32_t* words) {
     if (words == nullptr) return fail(GCMOE_ERR_INVALID, "null argument");
     cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
-    GCMOE_CUDA(cudaMemcpyFromSymbolAsync(words, g_producer_status, kStatusWords * 4, 0, cudaMemcpyDeviceToHost, s));
+    static std::mutex one_query;                       // of the process: they share the report
+    const std::lock_guard<std::mutex> lock(one_query);
+    take_producer_status_kernel<<<1, 1, 0, s>>>();
+    GCMOE_CUDA(cudaGetLastError());
+    GCMOE_CUDA(cudaMemcpyFromSymbolAsync(words, g_producer_report, kStatusWords * 4, 0, cudaMemcpyDeviceToHost, s));
     GCMOE_CUDA(cudaStreamSynchronize(s));
     if (words[kStatusCode] == 0) return GCMOE_OK;
-    static const uint32_t zero[kStatusWords] = {};
-    GCMOE_CUDA(cudaMemcpyToSymbolAsync(g_producer_status, zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s));
     return fail(GCMOE_ERR_DEVICE, "device wait gave up: code %u kernel %u site %u block %u observed %u expected %u",
                 words[kStatusCode], words[kStatusKernel], words[kStatusSite], words[kStatusBlock],
                 words[kStatusObserved], words[kStatusExpected]);

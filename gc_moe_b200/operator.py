@@ -12,6 +12,7 @@ from __future__ import annotations
 import ctypes
 import math
 import os
+import threading
 from typing import Optional, Tuple
 
 import torch
@@ -189,11 +190,31 @@ def check_plan_status(plan: _Plan) -> None:
     _native.raise_for(_native.library().gcmoe_status_read(plan.handle, ctypes.c_void_p(stream), words))
 
 
-def check_producer_status() -> None:
-    """Waits of the launches that have no plan (router logits)."""
+_producer_lock = threading.Lock()
+_producer_failures = {}          # device -> (number of failures read so far, message of the last)
+
+
+def producer_failures(device) -> int:
+    """Failures of plan-less launches (router logits) read on ``device`` so far."""
+    return _producer_failures.get(device, (0, ''))[0]
+
+
+def check_producer_status(sym_buffer, device) -> None:
+    """Waits of the launches that have no plan (router logits) on ``device``, the
+    current one.  The library reports a failure once, to whoever asks first, and
+    cannot tell whose launch it was: each workspace of the device hears of it once."""
     words = (ctypes.c_uint32 * _native.STATUS_WORDS)()
     stream = torch.cuda.current_stream().cuda_stream
-    _native.raise_for(_native.library().gcmoe_producer_status(ctypes.c_void_p(stream), words))
+    with _producer_lock:
+        code = _native.library().gcmoe_producer_status(ctypes.c_void_p(stream), words)
+        if code == _native.ERR_DEVICE:
+            _producer_failures[device] = (producer_failures(device) + 1, _native.last_error())
+        else:
+            _native.raise_for(code)
+        count, message = _producer_failures.get(device, (0, ''))
+        seen, sym_buffer._producer_failures_seen = sym_buffer._producer_failures_seen, count
+    if count > seen:
+        raise RuntimeError(message)
 
 
 def check_retired_status(scratch: torch.Tensor) -> None:

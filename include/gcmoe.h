@@ -232,9 +232,12 @@ typedef struct gcmoe_logits_args {
 int gcmoe_router_logits(const gcmoe_logits_args* args, void* cuda_stream);
 
 /* Status words of the bounded waits inside gcmoe_router_logits, after
- * synchronising `cuda_stream`: GCMOE_ERR_DEVICE if one of the launches on the
- * current device has given up since the last query (its part of the result is
- * NaN).  The launches have no plan, so the words live in the library. */
+ * synchronising `cuda_stream`: GCMOE_ERR_DEVICE if a launch on the current device
+ * has given up since the last query (its part of the result is NaN, which routing
+ * takes as masked: only this query tells it from a row without routes).  The
+ * launches have no plan, so the words live in the library, one set per device for
+ * the whole process: a query covers the launches that `cuda_stream` is ordered
+ * after, whoever made them, and clears what it reports. */
 int gcmoe_producer_status(void* cuda_stream, uint32_t* words);
 
 /* Test hook, as gcmoe_debug_expire_wait: one bounded wait that runs out and is
