@@ -952,7 +952,9 @@ static int launch_logits_mma(const gcmoe_logits_args& a, uint32_t split, cudaStr
 extern "C" int gcmoe_router_logits(const gcmoe_logits_args* args, void* cuda_stream) {
     if (args == nullptr) return fail(GCMOE_ERR_INVALID, "null argument");
     const gcmoe_logits_args& a = *args;
-    if (a.hidden == 0 || a.hidden % 8) return fail(GCMOE_ERR_INVALID, "hidden must be a positive multiple of 8");
+    // channels are coordinates of a tensor map, which are signed
+    if (a.hidden == 0 || a.hidden % 8 || a.hidden > (1u << 30))
+        return fail(GCMOE_ERR_INVALID, "hidden must be a positive multiple of 8 up to 2^30");
     if (a.num_experts == 0 || a.num_experts > uint32_t(kMaxExperts))
         return fail(GCMOE_ERR_INVALID, "num_experts must be in 1..%d", kMaxExperts);
     if (a.planes != 1 && a.planes != 3) return fail(GCMOE_ERR_INVALID, "the router weight has 1 or 3 bf16 planes");
@@ -1071,6 +1073,7 @@ extern "C" int gcmoe_route(const gcmoe_route_args* args, void* cuda_stream) {
     if (a.topk > a.topk_groups * (a.num_experts / a.num_groups))
         return fail(GCMOE_ERR_INVALID, "topk %u exceeds the %u experts of %u groups", a.topk,
                     a.topk_groups * (a.num_experts / a.num_groups), a.topk_groups);
+    if (a.num_tokens > 0x7fffffffu) return fail(GCMOE_ERR_INVALID, "too many tokens");
     if (a.logit_type > kLogitF16) return fail(GCMOE_ERR_INVALID, "logits must be f32, bf16 or f16");
     if (!(a.scale >= -3.0e38f && a.scale <= 3.0e38f)) return fail(GCMOE_ERR_INVALID, "scale must be finite");
     RouteParams p = {};

@@ -55,6 +55,12 @@ bool is_rows(const at::Tensor& t, int64_t rows, int64_t columns, int device) {
 // Elements between rows; a single row has no stride of its own.
 uint64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
+// Counts are 32 bits wide below this binding; what does not fit is refused, not cut off.
+constexpr int64_t kMaxCount = 0x7fffffff;
+PyObject* refuse_tokens(int64_t tokens) {
+    return refuse("%lld tokens are too many: at most %lld", (long long)tokens, (long long)kMaxCount);
+}
+
 at::Tensor new_rows(int64_t rows, int64_t columns, at::ScalarType type, const at::Tensor& like) {
     return at::detail::empty_strided_cuda({rows, columns}, {columns, 1}, type, like.device());
 }
@@ -77,6 +83,7 @@ PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t count) {
     if (!is_rows(*x, tokens, hidden, device)) return refuse(kXMessage);
     if (hidden == 0 || hidden % 32 || hidden > 32768)
         return refuse("hidden %lld must be a positive multiple of 32 up to 32768", (long long)hidden);
+    if (tokens > kMaxCount) return refuse_tokens(tokens);
     const at::Tensor* const weight = tensor_of(args[1]);
     if (weight == nullptr || !is_float(*weight) || weight->dim() != 1 || weight->size(0) != hidden ||
         !on_device(*weight, device) || !weight->is_contiguous())
@@ -166,6 +173,8 @@ PyObject* router_logits(PyObject*, PyObject* const* args, Py_ssize_t count) {
         w->size(1) < 1 || w->size(1) > 2048 || w->size(2) != hidden || !on_device(*w, device) || !w->is_contiguous())
         return refuse("router_weight must be contiguous bfloat16 [1 or 3, E <= 2048, %lld] on the device of x; call "
                       "transform_router_weight_for_gc_moe first", (long long)hidden);
+    if (hidden > kMaxCount) return refuse("hidden %lld is too large", (long long)hidden);
+    if (tokens > kMaxCount) return refuse_tokens(tokens);
     const int64_t experts = w->size(1);
     at::Tensor out;
     if (args[2] == Py_None) {
@@ -202,6 +211,7 @@ PyObject* route(PyObject*, PyObject* const* args, Py_ssize_t count) {
         return refuse("logits must be a 2-D CUDA float32, bfloat16 or float16 tensor, contiguous in its last dimension");
     const int64_t tokens = logits->size(0), experts = logits->size(1);
     const int device = logits->get_device();
+    if (tokens > kMaxCount) return refuse_tokens(tokens);
     const long topk = PyLong_AsLong(args[1]), groups = PyLong_AsLong(args[4]), topk_groups = PyLong_AsLong(args[5]);
     a.scale = static_cast<float>(PyFloat_AsDouble(args[8]));
     if (PyErr_Occurred()) return nullptr;

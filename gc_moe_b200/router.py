@@ -58,7 +58,7 @@ def check_router_weight(router_weight, hidden, device) -> None:
 def router_logits_for_gc_moe(x: torch.Tensor, router_weight: torch.Tensor,
                              out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """FP32 ``x @ W.T`` [T, E] of BF16 ``x`` [T, H] (rows may have a stride, their
-    starts are 16-byte aligned, H is a multiple of 8, T at most 262140) and the planes of
+    starts are 16-byte aligned, H is a multiple of 8 up to 2^30, T at most 262140) and the planes of
     ``transform_router_weight_for_gc_moe`` [P, E, H]: exact products, FP32 sums
     in an order that depends on the sizes alone.  ``out``: the tensor to write,
     contiguous; it may start anywhere in its storage.

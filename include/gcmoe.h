@@ -226,8 +226,8 @@ typedef struct gcmoe_logits_args {
 
 /* out[t][e] = sum over planes p and channels c of x[t][c] * weight[p][e][c], f32
  * sums.  planes = 1: a bf16 router weight; planes = 3: an f32 weight split into
- * bf16 terms.  H a multiple of 8, E at most 2048, T at most 262140.  The reference
- * takes routing decisions as inputs (README.md:234-252).  Allocates nothing;
+ * bf16 terms.  H a multiple of 8 up to 2^30, E at most 2048, T at most 262140.  The
+ * reference takes routing decisions as inputs (README.md:234-252).  Allocates nothing;
  * capturable. */
 int gcmoe_router_logits(const gcmoe_logits_args* args, void* cuda_stream);
 
@@ -266,9 +266,9 @@ typedef struct gcmoe_route_args {
  * the topk_groups best of num_groups groups of consecutive experts, descending,
  * ties to the lower expert; weights from the scores without the bias.  Experts
  * with a logit or bias of -inf or NaN are never chosen; index -1 and weight 0
- * where none is left.  E at most 2048, k at most 32, at most 32 groups.  The
- * reference takes routing decisions as inputs (README.md:234-252; its tests use
- * a softmax over the k largest logits, tests/test_gc_moe.py:130-168).
+ * where none is left.  E at most 2048, k at most 32, at most 32 groups, T below
+ * 2^31.  The reference takes routing decisions as inputs (README.md:234-252; its
+ * tests use a softmax over the k largest logits, tests/test_gc_moe.py:130-168).
  * Allocates nothing; capturable. */
 int gcmoe_route(const gcmoe_route_args* args, void* cuda_stream);
 

@@ -77,3 +77,29 @@ def test_an_infinity_gives_what_the_formula_gives(tokens, experts, hidden, weigh
     assert bool(torch.isfinite(got[rows:]).all())
     if tokens > rows:
         assert _close(got[rows:].cuda(), x[rows:], w)
+
+
+def test_sizes_past_32_bits_are_refused():
+    """Counts that do not fit the library's 32 bits must not lose their upper half (views of one row: nothing large is
+    read, and a refusal allocates nothing)."""
+    rows = 2 ** 32 + 3
+    x = torch.zeros((1, 32), dtype=torch.bfloat16, device='cuda').expand(rows, 32)
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    with pytest.raises(ValueError, match='tokens'):
+        G.router_logits_for_gc_moe(x, torch.zeros((1, 1, 32), dtype=torch.bfloat16, device='cuda'))
+    with pytest.raises(ValueError, match='tokens'):
+        G.route_for_gc_moe(x[:, :4], 1)
+    with pytest.raises(ValueError, match='tokens'):
+        G.rms_norm_for_gc_moe(x, torch.ones(32, device='cuda'), normed=False)
+    assert torch.cuda.max_memory_allocated() < before + 2 ** 20
+
+
+def test_a_row_past_32_bits_is_refused():
+    wide = torch.empty((1, 2 ** 32 + 8), dtype=torch.bfloat16, device='cuda')
+    try:
+        with pytest.raises(ValueError, match='hidden'):
+            G.router_logits_for_gc_moe(wide, wide[None])
+    finally:
+        del wide
+        torch.cuda.empty_cache()
