@@ -103,6 +103,7 @@ def stage_normed_inputs_for_gc_moe(sym_buffer, x: torch.Tensor, norm_weight: tor
         raise ValueError('symmetric buffer has been destroyed')
     if topk_groups is None:
         topk_groups = num_groups
+    renormalize = bool(renormalize)
     device, experts, topk = x.get_device(), sym_buffer.num_experts, sym_buffer.num_topk
     check_router_weight(router_weight, sym_buffer.hidden, device)
     if router_weight.shape[1] != experts:

@@ -8,6 +8,7 @@ and routes in its tests with a softmax over the k largest logits
 
 from __future__ import annotations
 
+from operator import index
 from typing import Optional, Tuple
 
 import torch
@@ -71,6 +72,8 @@ def router_logits_for_gc_moe(x: torch.Tensor, router_weight: torch.Tensor,
 def check_routing(experts, topk, scoring, bias, num_groups, topk_groups, group_score, scale, device) -> None:
     """Raise for options that ``route_for_gc_moe`` would refuse, for callers that
     enqueue something before it."""
+    for count in (topk, num_groups, topk_groups):
+        index(count)                                     # TypeError for what is not a whole number, 2.0 among them
     if scoring not in _SCORINGS:
         raise ValueError(f'scoring must be one of {_SCORINGS}, got {scoring!r}')
     if group_score not in _GROUP_SCORES:

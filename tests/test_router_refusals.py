@@ -1,10 +1,13 @@
-"""What the operators in front of the layer refuse before anything runs; no GPU
-needed."""
+"""What the operators in front of the layer refuse before anything runs; only the
+test marked ``gpu`` needs a GPU."""
 import ctypes
 
 import pytest
+import torch
 
+import gc_moe_b200 as G
 from gc_moe_b200 import _native, build
+from gc_moe_b200.router import check_routing
 
 
 @pytest.fixture(scope='module')
@@ -28,3 +31,32 @@ def test_counts_beyond_the_kernels_reach(lib):
             (lib.gcmoe_router_logits, _native.LogitsArgs, logits, dict(num_tokens=1, hidden=2 ** 32 - 8), 'hidden')):
         assert fn(ctypes.byref(struct(**{**good, **bad})), None) == _native.ERR_INVALID, bad
         assert word in _native.last_error(), _native.last_error()
+
+
+@pytest.mark.parametrize('change', [dict(topk=8.0), dict(num_groups=8.0), dict(topk_groups=4.0), dict(topk_groups='4'),
+                                    dict(num_groups=None), dict(scale='1'), dict(scale=None)])
+def test_options_of_another_kind(change):
+    """The check that stands in front of the norm refuses what the routing's call behind it would refuse."""
+    good = dict(experts=256, topk=8, scoring='sigmoid', bias=None, num_groups=8, topk_groups=4, group_score='top2',
+                scale=1.0, device=-1)
+    check_routing(**good)
+    with pytest.raises(TypeError):
+        check_routing(**{**good, **change})
+
+
+@pytest.mark.gpu
+def test_options_of_another_kind_leave_the_residual_alone(single_rank_group):
+    buf = G.get_symm_buffer_for_gc_moe(single_rank_group, 8, 256, 2, 1024, 512)
+    try:
+        x = torch.randn((4, 1024), device='cuda').to(torch.bfloat16)
+        residual, w = x * 2, torch.ones(1024, device='cuda')
+        planes = G.transform_router_weight_for_gc_moe(torch.zeros((8, 1024), dtype=torch.bfloat16, device='cuda'))
+        before = residual.clone()
+        for bad in (dict(num_groups=4, topk_groups=2.0), dict(num_groups=4.0), dict(scale='2'),
+                    dict(renormalize=torch.ones(2))):
+            with pytest.raises((TypeError, RuntimeError)):
+                G.stage_normed_inputs_for_gc_moe(buf, x, w, planes, residual, residual_out=residual, **bad)
+        torch.cuda.synchronize()
+        assert torch.equal(residual, before)
+    finally:
+        buf.destroy()
