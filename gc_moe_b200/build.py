@@ -29,21 +29,30 @@ def _newest_source_mtime() -> float:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile what is missing or older than its sources; the library's path."""
+    """Compile what is missing, older than its sources or (the binding) made for
+    another torch or Python; the library's path."""
+    library = _build_library(force, verbose)
     _build_binding(force)
-    return _build_library(force, verbose)
+    return library
 
 
 def _build_binding(force: bool) -> None:
-    if (not force and os.path.exists(BINDING)
-            and os.path.getmtime(BINDING) >= max(os.path.getmtime(f) for f in (BINDING_SOURCE, HEADER))):
-        return
     import sysconfig
     import torch
+    # An extension works with the torch and the Python it was made for; a note beside it says which.
+    made_for = f'torch {torch.__version__}, {sysconfig.get_config_var("SOABI")}'
+    note = os.path.splitext(BINDING)[0] + '.made_for'
+    if (not force and os.path.exists(BINDING) and os.path.exists(note) and open(note).read() == made_for
+            and os.path.getmtime(BINDING) >= max(os.path.getmtime(f) for f in (BINDING_SOURCE, HEADER))):
+        return
+    if os.path.exists(note):
+        os.remove(note)
     torch_dir = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(shutil.which('nvcc') or '/usr/local/cuda/bin/nvcc'))
     include = [os.path.join(torch_dir, 'include'), os.path.join(torch_dir, 'include', 'torch', 'csrc', 'api', 'include'),
                sysconfig.get_paths()['include'], os.path.join(cuda, 'include')]
+    if shutil.which('g++') is None:
+        raise RuntimeError('g++ not found; _torch_binding.so cannot be built')
     cmd = ['g++', '-O2', '-std=c++17', '-shared', '-fPIC',
            f'-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}', *(f'-isystem{i}' for i in include),
            BINDING_SOURCE, '-o', BINDING, f'-L{os.path.join(torch_dir, "lib")}',
@@ -51,6 +60,8 @@ def _build_binding(force: bool) -> None:
     result = subprocess.run(cmd, capture_output=True, text=True)
     if result.returncode != 0:
         raise RuntimeError('g++ failed:\n' + result.stdout + result.stderr)
+    with open(note, 'w') as f:
+        f.write(made_for)
 
 
 def _build_library(force: bool, verbose: bool) -> str:
