@@ -35,7 +35,9 @@ __device__ __forceinline__ long long clock_cycles() {
 
 // Programmatic dependent launch.  `grid_dependency_wait` returns once every
 // kernel this launch depends on has finished and its writes are visible;
-// before it a kernel may only do work that reads nothing those kernels wrote.
+// before it a kernel may only do work that reads nothing those kernels wrote.  After it,
+// loads are coherent ones: the non-coherent path (ld.global.nc, __ldg) is for memory that
+// nobody writes during the kernel, and this kernel may have started while those still wrote.
 // `launch_dependents` lets the next kernel of the stream start its own
 // prologue while this one is still running.
 __device__ __forceinline__ void grid_dependency_wait() {

@@ -172,12 +172,12 @@ __global__ void __launch_bounds__(kNormThreads, kChunks <= 2 ? 2 : 1) rms_norm_k
         float w[8] = {};
         if (in) {
             if constexpr (kWeightF32) {
-                const float4 a = __ldg(static_cast<const float4*>(p.weight) + 2 * c);
-                const float4 b = __ldg(static_cast<const float4*>(p.weight) + 2 * c + 1);
+                const float4 a = __ldca(static_cast<const float4*>(p.weight) + 2 * c);
+                const float4 b = __ldca(static_cast<const float4*>(p.weight) + 2 * c + 1);
                 w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
                 w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
             } else {
-                unpack_bf16x8(__ldg(static_cast<const uint4*>(p.weight) + c), w);
+                unpack_bf16x8(__ldca(static_cast<const uint4*>(p.weight) + c), w);
             }
         }
         float amax = 0.f;

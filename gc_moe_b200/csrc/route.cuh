@@ -106,7 +106,7 @@ __device__ __forceinline__ void load_run(const T* from, float (&v)[kCount]) {
     constexpr int kPer = int(sizeof(Vec) / sizeof(T));
 #pragma unroll
     for (int i = 0; i < kCount / kPer; ++i) {
-        const Vec raw = __ldg(reinterpret_cast<const Vec*>(from) + i);
+        const Vec raw = __ldca(reinterpret_cast<const Vec*>(from) + i);
         T part[kPer];
         memcpy(part, &raw, sizeof(Vec));
 #pragma unroll

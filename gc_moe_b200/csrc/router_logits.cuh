@@ -68,11 +68,11 @@ __global__ void __launch_bounds__(kLogitsThreads, kFmaResident<kTokens, kPlanes>
             const uint32_t c = c0 + r * kLogitsThreads;
             const bool in = c < chunks;
 #pragma unroll
-            for (int i = 0; i < kTokens; ++i) xr[r][i] = in ? __ldg(x[i] + c) : make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < kTokens; ++i) xr[r][i] = in ? __ldca(x[i] + c) : make_uint4(0, 0, 0, 0);
 #pragma unroll
             for (int e = 0; e < kExperts; ++e)
 #pragma unroll
-                for (int q = 0; q < kPlanes; ++q) wr[r][e][q] = in ? __ldg(w[e] + q * plane + c) : make_uint4(0, 0, 0, 0);
+                for (int q = 0; q < kPlanes; ++q) wr[r][e][q] = in ? __ldca(w[e] + q * plane + c) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int r = 0; r < kRounds; ++r)

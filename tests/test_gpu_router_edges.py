@@ -103,3 +103,51 @@ def test_a_row_past_32_bits_is_refused():
     finally:
         del wide
         torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize('tokens', [1, 4, 8, 40])
+@pytest.mark.parametrize('experts', [64, 256])
+def test_launches_in_flight_read_what_the_launch_before_wrote(tokens, experts):
+    """Products and routings one behind the other over ONE tensor of logits, each launched while those before it still
+    run: every routing reads the product directly before it, not an earlier content of the tensor."""
+    steps = 60
+    g = torch.Generator().manual_seed(tokens)
+    x = torch.randn((steps, tokens, 1024), generator=g).to(torch.bfloat16).cuda()
+    planes = G.transform_router_weight_for_gc_moe(torch.randn((experts, 1024), generator=g).cuda() * 0.03)
+    weight = torch.ones(1024, device='cuda')
+    want = []
+    for step in range(steps):
+        normed = G.rms_norm_for_gc_moe(x[step], weight).normed
+        torch.cuda.synchronize()
+        logits = G.router_logits_for_gc_moe(normed, planes)
+        torch.cuda.synchronize()
+        want.append([t.clone() for t in G.route_for_gc_moe(logits, 8)])
+        torch.cuda.synchronize()
+    logits = torch.zeros((tokens, experts), device='cuda')
+    normed = torch.zeros((tokens, 1024), dtype=torch.bfloat16, device='cuda')
+    out = [tuple(torch.zeros_like(t) for t in pair) for pair in want]
+
+    def chain(with_norm):
+        for step in range(steps):
+            rows = x[step]
+            if with_norm:
+                rows = G.rms_norm_for_gc_moe(x[step], weight, normed=normed).normed
+            else:
+                rows = ready[step]
+            G.router_logits_for_gc_moe(rows, planes, out=logits)
+            G.route_for_gc_moe(logits, 8, out=out[step])
+
+    ready = [G.rms_norm_for_gc_moe(x[step], weight).normed for step in range(steps)]
+    for with_norm in (True, False):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            chain(with_norm)
+        for run in (graph.replay, lambda: chain(with_norm)):
+            for _ in range(20):
+                for pair in out:
+                    for t in pair:
+                        t.zero_()
+                run()
+                torch.cuda.synchronize()
+                for got, ref in zip(out, want):
+                    assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
