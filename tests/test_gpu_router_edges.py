@@ -151,3 +151,44 @@ def test_launches_in_flight_read_what_the_launch_before_wrote(tokens, experts):
                 torch.cuda.synchronize()
                 for got, ref in zip(out, want):
                     assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
+
+
+# Tokens, experts, H: the form for few tokens with one, two and four of them a CTA and rows of one,
+# two and four rounds of loads, then each tile of the tensor-core form with each split of the K range.
+SIZES = [(1, 8, 2048), (2, 256, 4096), (3, 100, 7168), (8, 64, 4104), (8, 384, 2048),
+         (9, 8, 64), (64, 8, 512), (9, 8, 1024), (9, 512, 1024), (150, 384, 512), (300, 384, 2048), (700, 512, 64),
+         (512, 512, 512), (65, 512, 512), (65, 256, 1024), (2048, 384, 64), (700, 512, 1024), (300, 512, 2048),
+         (96, 512, 7168), (1000, 384, 2048), (300, 512, 7168), (64, 256, 7168), (33, 4, 1032)]
+
+
+@pytest.mark.parametrize('tokens,experts,hidden', SIZES)
+def test_each_plane_takes_part_in_full(tokens, experts, hidden):
+    """Planes of one size, one at a time and all together: in a real FP32 weight the third is below 2^-17 of the first,
+    and its loss would drown in the bound of the sum."""
+    g = torch.Generator(device='cuda').manual_seed(tokens + hidden)
+    x = torch.randn((tokens, hidden), generator=g, device='cuda').to(torch.bfloat16)
+    planes = torch.randn((3, experts, hidden), generator=g, device='cuda').to(torch.bfloat16)
+    for kept in ((0,), (1,), (2,), (0, 1, 2)):
+        some = torch.zeros_like(planes)
+        some[list(kept)] = planes[list(kept)]
+        got = G.router_logits_for_gc_moe(x, some)
+        want = sum(x.double() @ p.double().T for p in some)
+        size = sum(x.double().abs() @ p.double().abs().T for p in some)
+        assert bool(((got.double() - want).abs() <= size * 2.0 ** -15).all()), kept
+
+
+@pytest.mark.parametrize('weight', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('tokens,experts,hidden', [(9, 8, 65536), (64, 256, 65536), (150, 384, 65536), (300, 256, 65536),
+                                                   (2048, 384, 7168), (4096, 256, 7168)])
+def test_truncation_does_not_grow_with_the_row(tokens, experts, hidden, weight):
+    """Terms of one sign, whose partial sums only grow.  A tensor core's addition loses less than 2^-23 of its partial
+    sum; in a chain of 512 channels, 32 additions, the partial sums are i/32 of the chain's: less than 16.5 * 2^-23
+    = 2.0e-6 of it, half of that on average.  The sums of the chains are rounded to nearest, which favours no side.
+    One chain over these rows (at least 3584 channels a CTA) would lose 3.9e-6 to 9e-6 on average."""
+    g = torch.Generator(device='cuda').manual_seed(experts)
+    x = (torch.rand((tokens, hidden), generator=g, device='cuda') + 0.5).to(torch.bfloat16)
+    w = (torch.rand((experts, hidden), generator=g, device='cuda') + 0.5).to(weight)
+    got = G.router_logits_for_gc_moe(x, G.transform_router_weight_for_gc_moe(w))
+    want = torch.cat([rows.double() @ w.double().T for rows in x.split(256)])
+    bias = float(((got.double() - want) / want).mean())
+    assert abs(bias) < 16.5 * 2.0 ** -23, bias
