@@ -275,12 +275,12 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
     // then all of them have started and, where the parts lie in the stages, are done with them.
     if constexpr (Tile::kApart) ptx::cluster_arrive_relaxed();
     ptx::grid_dependency_wait();
-    ptx::launch_dependents();
 
     uint32_t tmem = 0;
     if (warp >= 1 && warp < 10) {
-        // The loads start meanwhile.  TMEM only after the kernels before this one have ended:
-        // none of them can be waiting for it.
+        // The loads start meanwhile.  TMEM only after the kernels before this one have ended and
+        // before the ones behind it may start: one of those could hold TMEM of this SM until
+        // this kernel ends, and the allocation, which has no limit, would wait for it.
         if (warp == 1) {
             ptx::tmem_alloc<false>(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), Tile::kTmemColumns);
             ptx::tmem_relinquish<false>();
@@ -289,6 +289,7 @@ __global__ void __launch_bounds__(kLogitsMmaThreads, 1) logits_mma_kernel(const 
         asm volatile("bar.sync 1, 288;" ::: "memory");
         ptx::tc_fence_after();
         tmem = *tmem_slot;
+        ptx::launch_dependents();
     }
 
     float acc[kN / 2];                                                    // warps 2-9: one token, half of the experts

@@ -14,3 +14,17 @@ def test_no_non_coherent_loads():
     for path in sources:
         code = re.sub(r'//[^\n]*', '', open(path).read())
         assert '__ldg' not in code and not re.search(r'ld\.global(\.\w+)*\.nc', code), path
+
+
+def test_tensor_memory_is_allocated_before_dependents_may_start():
+    """A dependent that holds tensor memory of the SM waits for the end of the kernel that let it start; an allocation
+    behind that point could wait for the dependent, without end."""
+    found = 0
+    for path in glob.glob(os.path.join(CSRC, '*.cuh')):
+        code = re.sub(r'//[^\n]*', '', open(path).read())
+        if path.endswith('ptx.cuh') or 'ptx::tmem_alloc' not in code:
+            continue
+        body = code[code.rindex('__global__', 0, code.rindex('ptx::tmem_alloc')):]
+        assert body.index('ptx::tmem_alloc') < body.index('ptx::launch_dependents'), path
+        found += 1
+    assert found == 2
