@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(kLogitsThreads, kFmaResident<kTokens, kPlanes>
 // Bound by launch, load latency and the partial tiles' exchange for up to a few hundred
 // tokens (33 x 5120 x 384: 4.2 us, an empty launch 0.6), then by the MMAs (82
 // cycles for 128 x 128, 64 at best) and the traffic from L2 to the SMs: 4096 x 7168 x 256 takes
-// 18.7 us with 235 MB brought to the SMs; the inputs need 10.2 us of HBM.  Tiles of 256
+// 18.7 us (21.8 after a second of it) with 235 MB brought to the SMs; the inputs need 10.2 us of HBM.  Tiles of 256
 // experts, as one CTA or as a pair with 256 tokens, move half to two thirds of that but were
 // no faster at any size (20.8 and 22 us here): their shared memory holds too few stages to
 // cover the latency.  An MMA of 64 rows takes half the time of one of 128, and its smaller
@@ -142,7 +142,6 @@ __global__ void __launch_bounds__(kLogitsThreads, kFmaResident<kTokens, kPlanes>
 // Warp 0: loads of x; warp 1: MMAs; warps 2-9: accumulators to registers, then the sums;
 // warp 10: loads of W.
 constexpr uint32_t kLogitsMmaThreads = 352;
-constexpr uint32_t kLogitsMaxTokens = 128;           // of a tile
 constexpr uint32_t kLogitsBlockK = 64;
 constexpr uint32_t kChainBlocks = 8;
 

@@ -44,8 +44,8 @@ struct StageParams {
     uint32_t hidden, num_experts, topk;
 };
 
-// Biased exponent of the smallest power of two >= amax / 448 for a finite
-// non-negative amax whose mantissa has at most 7 fraction bits (BF16): 448 is
+// Biased exponent of the smallest power of two >= amax / 448 for any finite
+// non-negative f32 amax (a BF16 value here, an unrounded one in the norm): 448 is
 // 1.75 * 2^8, so the exponent goes up by one exactly when the mantissa exceeds
 // 1.75 (fraction 0x600000), and the result is floored at code 0 (2^-127).
 __device__ __forceinline__ uint32_t ue8m0_code_for_e4m3(float amax) {

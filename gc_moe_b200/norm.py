@@ -32,7 +32,7 @@ def rms_norm_for_gc_moe(x: torch.Tensor, weight: torch.Tensor, residual: Optiona
                         residual_out: Optional[torch.Tensor] = None, sym_buffer=None) -> NormedInputs:
     """``h = x + residual``; ``v = h / sqrt(mean(h * h) + eps) * weight``, all in
     FP32, from BF16 ``x`` [T, H], ``residual`` [T, H] and ``weight`` [H] (BF16 or
-    FP32 each; H a multiple of 32 up to 32768).
+    FP32 each; H a multiple of 32 up to 32768; the weight 16-byte aligned).
 
     Returns ``v`` as e4m3 rows with one UE8M0 scale ``2^ceil(log2(amax / 448))``
     per 32 channels (the layer's input format; rows and words of the workspace

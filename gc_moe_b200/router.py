@@ -24,11 +24,12 @@ def transform_router_weight_for_gc_moe(weight: torch.Tensor) -> torch.Tensor:
     """Router weight [E, H] -> the BF16 planes [P, E, H] that
     ``router_logits_for_gc_moe`` reads; their sum is the weight.
 
-    A BF16 weight is its own single plane (no copy when it is contiguous).  The
-    24 significant bits of an FP32 weight are three planes of 8: the nearest BF16,
-    the BF16 nearest to what is left, and the rest; planes that would be zero
-    (a BF16 weight stored as FP32) are left out.  Call once per weight, outside
-    graph capture.
+    A BF16 weight is its own single plane (no copy when it is contiguous; it then
+    has to start on 16 bytes).  The 24 significant bits of an FP32 weight are three
+    planes of 8: the nearest BF16, the BF16 nearest to what is left, and the rest.
+    The product takes one plane or three: a weight of BF16 values stored in FP32
+    is one, FP16's 11 bits are three, the last of them zero.  Call once per
+    weight, outside graph capture.
     """
     if weight.dim() != 2 or weight.dtype not in _WEIGHT_TYPES:
         raise ValueError('router weight must be 2-D bfloat16, float16 or float32')
@@ -59,12 +60,15 @@ def check_router_weight(router_weight, hidden, device) -> None:
 def router_logits_for_gc_moe(x: torch.Tensor, router_weight: torch.Tensor,
                              out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """FP32 ``x @ W.T`` [T, E] of BF16 ``x`` [T, H] (rows may have a stride, their
-    starts are 16-byte aligned, H is a multiple of 8 up to 2^30, T at most 262140) and the planes of
-    ``transform_router_weight_for_gc_moe`` [P, E, H]: exact products, FP32 sums
-    in an order that depends on the sizes alone.  ``out``: the tensor to write,
-    contiguous; it may start anywhere in its storage.
+    starts are 16-byte aligned, H is a multiple of 8 up to 2^30, T at most 262140)
+    and the planes of ``transform_router_weight_for_gc_moe`` [P, E, H]: exact
+    products, FP32 sums in an order that depends on the sizes alone.  An infinity
+    in ``x`` gives what it gives times the weight itself, whatever the planes.
+    ``out``: the tensor to write, contiguous; it may start anywhere in its storage.
 
-    Runs on the current stream and can be captured.
+    Runs on the current stream and can be captured.  A launch whose bounded wait
+    gives up leaves NaN, which routing takes as masked: only
+    ``GCSymmBuffer.raise_on_device_error`` tells it from a row without routes.
     """
     return _native.binding().router_logits(x, router_weight, out)
 
